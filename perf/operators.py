@@ -47,30 +47,30 @@ def listed():
 
     return [
         # the token of a decode step enters the cache (the smallest call)
-        named("store 1 token, 4 bit", "store", 4, 8, 2, 256, 1, 1040),
+        named("store 1 token 4bit", "store", 4, 8, 2, 256, 1, 1040),
         # the benchmark's prompt length, less a ragged end, as a projection
         # leaves it (token-major)
-        named("store 1000 tokens, 8 bit", "store", 8, 8, 2, 256, 1, 1000, new=1000, token_major=True),
+        named("store 1000 tokens 8bit", "store", 8, 8, 2, 256, 1, 1000, new=1000, token_major=True),
         # a bf16 cache of a long document moves into the small one
-        named("store 100003 tokens, 4 bit", "store", 4, 8, 2, 256, 1, 100003, new=100003),
+        named("store 100003 tokens 4bit", "store", 4, 8, 2, 256, 1, 100003, new=100003),
         # a chat's cache is read back to go on in bf16
-        named("load 777 tokens, 4 bit", "load", 4, 8, 2, 256, 1, 777),
+        named("load 777 tokens 4bit", "load", 4, 8, 2, 256, 1, 777),
         # a long document's cache is read back
-        named("load 131072 tokens, 8 bit", "load", 8, 8, 2, 256, 1, 131072),
+        named("load 131072 tokens 8bit", "load", 8, 8, 2, 256, 1, 131072),
         # a decode step at the benchmark's context, with the output gate
-        named("decode ctx 1088, 4 bit", "decode", 4, 8, 2, 256, 1, 1088, gate=True),
+        named("decode ctx 1088 4bit", "decode", 4, 8, 2, 256, 1, 1088, gate=True),
         # a decode step over a document
-        named("decode ctx 16001, 8 bit", "decode", 8, 8, 2, 256, 1, 16001, gate=True),
+        named("decode ctx 16001 8bit", "decode", 8, 8, 2, 256, 1, 16001, gate=True),
         # a decode step over the longest context
-        named("decode ctx 131071, 4 bit", "decode", 4, 8, 2, 256, 1, 131071),
+        named("decode ctx 131071 4bit", "decode", 4, 8, 2, 256, 1, 131071),
         # a served batch of unequal contexts, one slot of it unused
-        named("decode 16 x 8000, 4 bit", "decode", 4, 32, 8, 128, 16, 8000),
+        named("decode 16 x 8000 4bit", "decode", 4, 32, 8, 128, 16, 8000),
         # a few drafted tokens are checked over a document
-        named("prompt 5 after 8192, 4 bit", "prompt", 4, 8, 2, 256, 1, 8197, new=5),
+        named("prompt 5 after 8192 4bit", "prompt", 4, 8, 2, 256, 1, 8197, new=5),
         # a prompt of ordinary length
-        named("prompt 1000, 4 bit", "prompt", 4, 8, 2, 256, 1, 1000, new=1000),
+        named("prompt 1000 4bit", "prompt", 4, 8, 2, 256, 1, 1000, new=1000),
         # the next part of a long document
-        named("prompt 4096 after 28000, 8 bit", "prompt", 8, 8, 2, 256, 1, 32096, new=4096),
+        named("prompt 4096 after 28000 8bit", "prompt", 8, 8, 2, 256, 1, 32096, new=4096),
     ]
 
 
