@@ -24,7 +24,7 @@ extern "C" {
 #endif
 
 /* ABI version of this header; q35_abi_version() must return it. */
-#define Q35_ABI_VERSION 5
+#define Q35_ABI_VERSION 6
 int q35_abi_version(void);
 
 /* Zero n device buffers in one launch per 128: ptrs[i] (16-byte aligned) holds
@@ -452,6 +452,52 @@ int q35_dequant_swiglu_quant(const void* acc, const void* s_x, const void* s_w, 
  * q35_gemv_a8w8, replacing the output stage of explore_runtime_quantization.py:173-180. */
 int q35_dequant_i32(const void* acc, const void* s_x, const void* s_w, void* y, int M, int N,
                     void* stream);
+
+/* ---- K/V cache in 4 or 8 bits ---------------------------------------- */
+/* No counterparts among the reference's kernels: its static cache is bf16.
+ *
+ * Rows of one head (D = 64, 128 or 256) in groups of 64 values, a group as low
+ * + step * code: low its least value (bf16), step = bf16((greatest - low) / (2^
+ * bits - 1)), code the whole number nearest to (x - low) / step (ties to even,
+ * decided in the real numbers), 0 .. 2^bits - 1. A group without a range has
+ * step 0 and codes 0; one that holds a NaN or an infinity reads back as NaN.
+ * Keys: group g is dims 64 g .. 64 g + 63; values: group g is the dims d with
+ * (d mod D/16) div 4 == g.
+ *
+ * kq, vq: codes [B, KVH, capacity, D * bits / 8] bytes, dims in order, in 4
+ * bits the even dim in a byte's low half. kp, vp: [B, KVH, D / 64, capacity]
+ * pairs of bf16, step then low. All 16-byte aligned, capacity % 32 == 0,
+ * capacity * D * bits / 8 < 2^31. */
+
+/* Quantise L rows a head of k and v (bf16, element strides of batch, head and
+ * token; the dims of a row contiguous; base and strides 16-byte aligned, for D
+ * = 64 8-byte) into positions start_b + start .. of the cache, start_b =
+ * start_dev[b] (int64, n_start = B or 1 shared one) or 0 when start_dev is
+ * null. Positions outside the cache are not written. */
+int q35_kv_quantize(const void* k, long long k_sb, long long k_sh, long long k_sl, const void* v,
+                    long long v_sb, long long v_sh, long long v_sl, void* kq, void* vq, void* kp,
+                    void* vp, const void* start_dev, int n_start, long long start, int B, int KVH,
+                    int L, int D, int bits, int capacity, void* stream);
+/* Positions start .. start + L - 1 as bf16 k, v [B, KVH, L, D] (16-byte
+ * aligned): bf16(low + step * code), one rounding. */
+int q35_kv_dequantize(const void* kq, const void* vq, const void* kp, const void* vp, void* k,
+                      void* v, int start, int B, int KVH, int L, int D, int bits, int capacity,
+                      void* stream);
+/* Causal GQA attention over the cache: q [B, QH, L, D] bf16, query row i of
+ * sequence b sees the keys at positions 0 .. s_b + i, s_b = len_dev[b] + offset
+ * (int64, n_len = B or 1 shared one; 0 + offset when len_dev is null), within
+ * the capacity; a row that sees none is zero. out [B, L, QH * D] bf16. gate (L
+ * == 1 only, 8-byte aligned, rows gate_stride elements apart, [q | gate] per
+ * query head as the packed QGKV row): out times sigmoid(gate). Workspace:
+ * q35_gqa_attention_kvq_workspace floats (-1 for sizes the entry refuses), not
+ * shared by launches that overlap in time. */
+long long q35_gqa_attention_kvq_workspace(int B, int QH, int KVH, int L, int D, int bits,
+                                          int capacity);
+int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const void* kp,
+                          const void* vp, const void* len_dev, int n_len, long long offset,
+                          const void* gate, long long gate_stride, float scale, void* out,
+                          void* workspace, long long workspace_floats, int B, int QH, int KVH, int L,
+                          int D, int bits, int capacity, void* stream);
 
 /* ---------------------------------------------------------- vision encoder */
 /* Vision LayerNorm over rows of `width`: y = bf16((x - mean) * rsqrt(var +

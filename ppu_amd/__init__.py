@@ -8,16 +8,22 @@ the reference's import names.
 """
 
 from .kernels import (  # noqa: F401
+    QuantizedKV,
     attention_gate_mul,
     causal_conv1d_fused,
     delta_recurrent_fused,
     gated_rms_norm,
     gqa_decode_attention,
+    gqa_decode_attention_q,
+    gqa_prefill_attention_q,
+    kv_cache_dequantize,
+    kv_cache_quantize,
     layer_norm,
     lm_head_argmax,
     position_embed_add,
     ppu_swiglu_gemv,
     qgkv_norm_rope,
+    quantized_kv_cache,
     residual_add_layer_norm,
     residual_add_rms_norm,
     rms_norm,

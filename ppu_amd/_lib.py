@@ -14,7 +14,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().with_name("libq35.so")
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -98,6 +98,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "q35_host_device_ptr": (_I, [_P, _P]),
     "q35_attn_gate_quant": (_I, [_P, _P, _P, _P, _L, _I, _I, _I, _P, _L, _P]),
     "q35_embed_rmsnorm": (_I, [_P, _I, _P, _P, _I, _P, _P, _I, _I, _F, _P]),
+    "q35_kv_quantize": (
+        _I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _P, _I, _L, _I, _I, _I, _I, _I, _I, _P]),
+    "q35_kv_dequantize": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "q35_gqa_attention_kvq_workspace": (_L, [_I, _I, _I, _I, _I, _I, _I]),
+    "q35_gqa_attention_kvq": (
+        _I, [_P, _P, _P, _P, _P, _P, _I, _L, _P, _L, _F, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _P]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import functools
 import itertools
+from typing import NamedTuple
 
 import torch
 
@@ -1231,6 +1232,253 @@ def gqa_prefill_attention(
               offset if valid_length is not None else kv_start, _lib.ptr(valid_length),
               float(scale), _lib.ptr(ws), floats, _stream(q))
     return out
+
+
+# ------------------------------------------------------------------ K/V cache in 4 or 8 bits
+class QuantizedKV(NamedTuple):
+    """A static K/V cache in 4 or 8 bits (``quantized_kv_cache`` makes one).
+
+    ``keys`` / ``values``: codes, uint8 ``[B, KVH, C, D * bits / 8]``;
+    ``key_params`` / ``value_params``: bf16 ``[B, KVH, D / 64, C, 2]``, the
+    (step, low) of every group of 64 values, a value being ``low + step *
+    code``. Key group g is dims 64 g .. 64 g + 63, value group g the dims d with
+    ``(d mod D/16) div 4 == g``; in 4 bits the even dim is a byte's low half.
+    D is 64, 128 or 256; C a multiple of 32. 144 bytes a token and head of 256
+    in 4 bits, 272 in 8 bits, against 512 in bf16 (each for K and for V)."""
+
+    keys: torch.Tensor
+    values: torch.Tensor
+    key_params: torch.Tensor
+    value_params: torch.Tensor
+
+    @property
+    def head_dim(self) -> int:
+        return 64 * self.key_params.shape[2]
+
+    @property
+    def bits(self) -> int:
+        return self.keys.shape[3] * 8 // self.head_dim
+
+    @property
+    def capacity(self) -> int:
+        return self.keys.shape[2]
+
+
+def quantized_kv_cache(batch: int, kv_heads: int, capacity: int, head_dim: int, *, bits: int = 4,
+                       device: torch.device | str = "cuda") -> QuantizedKV:
+    """An empty cache of ``capacity`` positions (rounded up to a multiple of
+    32), all zeros, for ``kv_cache_quantize`` and the ``_q`` attentions."""
+
+    if bits not in (4, 8) or head_dim not in (64, 128, 256):
+        raise ValueError("a quantised K/V cache has 4 or 8 bits and heads of 64, 128 or 256")
+    if batch < 1 or kv_heads < 1 or capacity < 1:
+        raise ValueError("a quantised K/V cache needs at least one sequence, head and position")
+    capacity = (capacity + 31) // 32 * 32
+    codes = [torch.zeros((batch, kv_heads, capacity, head_dim * bits // 8), device=device, dtype=torch.uint8)
+             for _ in range(2)]
+    params = [torch.zeros((batch, kv_heads, head_dim // 64, capacity, 2), device=device, dtype=_BF16)
+              for _ in range(2)]
+    return QuantizedKV(*codes, *params)
+
+
+def _kvq_layout(cache: QuantizedKV) -> tuple[int, int, int, int, int]:
+    """Check a cache's form; ``(batch, KV heads, capacity, head dim, bits)``."""
+
+    kq, vq, kp, vp = cache
+    if kq.ndim != 4 or kp.ndim != 5 or vq.shape != kq.shape or vp.shape != kp.shape:
+        raise ValueError("quantised cache: codes [B,KVH,C,D*bits/8] and params [B,KVH,D/64,C,2], K as V")
+    if not (kq.dtype == vq.dtype == torch.uint8 and kp.dtype == vp.dtype == _BF16):
+        raise ValueError("quantised cache: uint8 codes and bfloat16 params")
+    batch, kv_heads, capacity, width = kq.shape
+    groups = kp.shape[2]
+    dim = 64 * groups
+    bits = width * 8 // dim if dim else 0
+    if groups not in (1, 2, 4) or bits not in (4, 8) or width * 8 != dim * bits:
+        raise ValueError("a quantised K/V cache has 4 or 8 bits and heads of 64, 128 or 256")
+    if kp.shape != (batch, kv_heads, groups, capacity, 2) or batch == 0 or kv_heads == 0:
+        raise ValueError("quantised cache: codes and params do not match")
+    if capacity == 0 or capacity % 32 or capacity * width >= 1 << 31:
+        raise ValueError("quantised cache capacity must be a multiple of 32 (and a head's codes below 2 GiB)")
+    if not (kq.is_contiguous() and vq.is_contiguous() and kp.is_contiguous() and vp.is_contiguous()):
+        raise ValueError("quantised cache tensors must be contiguous")
+    if (kq.data_ptr() | vq.data_ptr() | kp.data_ptr() | vp.data_ptr()) % 16:
+        raise ValueError("quantised cache tensors must be 16-byte aligned")
+    return batch, kv_heads, capacity, dim, bits
+
+
+def _kvq_positions(t: torch.Tensor | None, batch: int, name: str) -> int:
+    """Check an int64 tensor of one position or one per sequence; its count."""
+
+    if t is None:
+        return 0
+    n = t.numel()
+    if t.dtype != torch.int64 or n not in (1, batch) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int64 tensor of one value, or one per sequence")
+    return n
+
+
+def _kvq_call(name: str, cache: QuantizedKV, operands: tuple, *args) -> None:
+    """Launch on the current stream of the cache's GPU, which need not be the
+    current GPU; every operand has to be there."""
+
+    device = cache[0].device
+    if device.type != "cuda":
+        raise ValueError(f"fused kernels require GPU tensors: the cache is on {device}")
+    for t in (*cache[1:], *operands):
+        if t is not None and t.device != device:
+            raise ValueError(f"fused kernels require tensors of one GPU: {t.device}, the cache on {device}")
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, _lib.stream(device))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _lib.stream(device))
+
+
+def _kvq_rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows as the write kernel reads them: dims contiguous, 16-byte loads
+    (8-byte for heads of 64); anything else is copied."""
+
+    unit = 8 if t.shape[3] > 64 else 4
+    s = t.stride()
+    if s[3] == 1 and (s[0] | s[1] | s[2]) % unit == 0 and t.data_ptr() % (2 * unit) == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def kv_cache_quantize(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cache: QuantizedKV,
+    *,
+    start: int = 0,
+    cache_start: torch.Tensor | None = None,
+) -> None:
+    """Quantise ``k, v [B, KVH, L, D]`` (bf16; any strides, e.g. views of a
+    token-major projection) into positions ``start .. start + L - 1`` of the
+    cache. With ``cache_start`` (int64 on the GPU, one value or one per
+    sequence, as a static cache's length) the positions start there instead and
+    those outside the cache are not written. Every group of 64 values is
+    rounded on its own (``QuantizedKV``); one that holds a NaN or an infinity
+    reads back as NaN."""
+
+    batch, kv_heads, capacity, dim, bits = _kvq_layout(cache)
+    if k.ndim != 4 or k.shape != v.shape or k.shape[:2] != (batch, kv_heads) or k.shape[3] != dim:
+        raise ValueError(f"k and v must be [{batch},{kv_heads},L,{dim}] as the cache")
+    _need_bf16(k, v)
+    length = k.shape[2]
+    n_start = _kvq_positions(cache_start, batch, "cache_start")
+    if cache_start is not None and start:
+        raise ValueError("start and cache_start are exclusive")
+    if cache_start is None and (start < 0 or start + length > capacity):
+        raise ValueError("rows exceed the quantised cache")
+    k, v = _kvq_rows(k), _kvq_rows(v)
+    kq, vq, kp, vp = cache
+    _kvq_call("q35_kv_quantize", cache, (k, v, cache_start), k.data_ptr(), *k.stride()[:3], v.data_ptr(),
+              *v.stride()[:3], kq.data_ptr(), vq.data_ptr(), kp.data_ptr(), vp.data_ptr(),
+              _lib.ptr(cache_start), n_start, start, batch, kv_heads, length, dim, bits, capacity)
+
+
+def kv_cache_dequantize(cache: QuantizedKV, length: int, *, start: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Positions ``start .. start + length - 1`` of the cache as bf16 ``k, v
+    [B, KVH, length, D]``: ``low + step * code``, rounded once."""
+
+    batch, kv_heads, capacity, dim, bits = _kvq_layout(cache)
+    if start < 0 or length < 0 or start + length > capacity:
+        raise ValueError("rows exceed the quantised cache")
+    kq, vq, kp, vp = cache
+    k = torch.empty((batch, kv_heads, length, dim), device=kq.device, dtype=_BF16)
+    v = torch.empty_like(k)
+    _kvq_call("q35_kv_dequantize", cache, (), kq.data_ptr(), vq.data_ptr(), kp.data_ptr(), vp.data_ptr(),
+              k.data_ptr(), v.data_ptr(), start, batch, kv_heads, length, dim, bits, capacity)
+    return k, v
+
+
+def _kvq_attention(q, cache, layout, lengths, offset, scale, gate):
+    batch, kv_heads, capacity, dim, bits = layout
+    heads, length = q.shape[1], q.shape[2]
+    n_len = _kvq_positions(lengths, batch, "valid_length")
+    if q.data_ptr() % 16:
+        q = q.clone()
+    out = torch.empty((batch, length, heads * dim), device=q.device, dtype=_BF16)
+    floats = _lib.load().q35_gqa_attention_kvq_workspace(batch, heads, kv_heads, length, dim, bits, capacity)
+    ws = torch.empty(floats, device=q.device, dtype=torch.float32) if floats > 0 else None
+    kq, vq, kp, vp = cache
+    _kvq_call("q35_gqa_attention_kvq", cache, (q, lengths, gate), q.data_ptr(), kq.data_ptr(), vq.data_ptr(),
+              kp.data_ptr(), vp.data_ptr(), _lib.ptr(lengths), n_len, offset, _lib.ptr(gate),
+              0 if gate is None else gate.shape[-1], float(scale), out.data_ptr(), _lib.ptr(ws), floats,
+              batch, heads, kv_heads, length, dim, bits, capacity)
+    return out
+
+
+def _kvq_query(q: torch.Tensor, layout) -> None:
+    batch, kv_heads, _, dim, _ = layout
+    if q.ndim != 4 or q.shape[0] != batch or q.shape[3] != dim or q.shape[1] == 0 or q.shape[1] % kv_heads:
+        raise ValueError("attention head layout does not match the quantised cache")
+    if not q.is_contiguous():
+        raise ValueError("attention queries must be contiguous")
+    _need_bf16(q)
+
+
+def gqa_decode_attention_q(
+    q: torch.Tensor,
+    cache: QuantizedKV,
+    valid_length: torch.Tensor,
+    scale: float,
+    *,
+    packed_gate: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``gqa_decode_attention`` over a cache in 4 or 8 bits: one token of every
+    sequence, ``q [B, H, 1, D]``, attends to the first ``valid_length`` (int64
+    on the GPU, one value or one per sequence, the current token included)
+    positions. With ``packed_gate`` (the packed QGKV rows ``[B, 1, P]``) the
+    result is multiplied by the sigmoid of each head's gate. ``[B, 1, H*D]``
+    bf16, rounded once; zeros for a sequence without valid positions."""
+
+    layout = _kvq_layout(cache)
+    _kvq_query(q, layout)
+    if q.shape[2] != 1:
+        raise ValueError("GQA decode attention expects q[B,H,1,D]")
+    if packed_gate is not None:
+        width = packed_gate.shape[-1]
+        if (width < 2 * q.shape[1] * q.shape[3] or width % 4 or packed_gate.numel() != layout[0] * width
+                or not packed_gate.is_contiguous() or packed_gate.data_ptr() % 8):
+            raise ValueError("packed gate does not match the attention heads")
+        _need_bf16(packed_gate)
+    return _kvq_attention(q, cache, layout, valid_length, -1, scale, packed_gate)
+
+
+def gqa_prefill_attention_q(
+    q: torch.Tensor,
+    cache: QuantizedKV,
+    scale: float,
+    *,
+    kv_start: int = 0,
+    valid_length: torch.Tensor | None = None,
+    length_is_start: bool = False,
+) -> torch.Tensor:
+    """``gqa_prefill_attention`` over a cache in 4 or 8 bits, which already
+    holds the keys and values of the L tokens (``kv_cache_quantize``): row i of
+    ``q [B, QH, L, D]`` attends to positions ``[0, start + i]``, with ``start =
+    valid_length - L`` (int64 on the GPU, one value or one per sequence), ``start
+    = valid_length`` with ``length_is_start``, else ``kv_start``. Positions past
+    the capacity do not exist, and a row that sees none (a negative start, as
+    the padding rows of a left-padded batch have) is zero. ``[B, L, QH*D]``
+    bf16."""
+
+    layout = _kvq_layout(cache)
+    _kvq_query(q, layout)
+    capacity, length = layout[2], q.shape[2]
+    if valid_length is None:
+        if length_is_start:
+            raise ValueError("length_is_start needs valid_length")
+        if kv_start < 0 or kv_start + length > capacity:
+            raise ValueError("prefill attention range exceeds the key/value length")
+    elif kv_start:
+        raise ValueError("kv_start and valid_length are exclusive")
+    if length > capacity:
+        raise ValueError("prefill attention range exceeds the key/value length")
+    offset = kv_start if valid_length is None else 0 if length_is_start else -length
+    return _kvq_attention(q, cache, layout, valid_length, offset, scale, None)
 
 
 # ------------------------------------------------------------------ A8W8
