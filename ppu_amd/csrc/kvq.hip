@@ -19,7 +19,9 @@
 // Layouts: codes [B, KVH, C, D * bits / 8] bytes, dims in order, in 4 bits the
 // even dim in a byte's low half; params [B, KVH, D / 64, C] pairs of bf16
 // (step in the low half of a 32-bit word, low in the high half).
-#include "q35_common.hpp"
+#include <type_traits>
+
+#include "q35_tile.hpp"
 
 namespace {
 
@@ -278,6 +280,498 @@ __global__ __launch_bounds__(256) void kvq_attend_rows(
   }
 }
 
+// ------------------------------------------------- attention of a few rows
+// The query rows of one KV head, G = QH / KVH heads x L tokens, in blocks of HP
+// rows; a workgroup takes one block and every S-th piece of NW x 32 keys, a
+// wave one tile of 32 keys of each piece. Products are transposed, keys or dims
+// as the rows of v_mfma_f32_16x16x32_bf16 and query rows as its columns, and a
+// column is a pair (query row, group): the 16 columns are HP rows x GT of the
+// NG groups, CT = NG / GT column tiles in all. A lane then needs one step and
+// one low per key, its own group's:
+//   S^T[key, (row, group)] = step (K' Q^T + mid' Q sums), K' = the codes (less
+//     half their range) and Q zero outside the column's group; the groups'
+//     parts are added over GT neighbouring lanes. The MFMA accumulates from -c
+//     sum(q), c the offset of the codes as bf16: 4-bit codes become 16 + code by
+//     one shift and one and-or for two of them (24 is taken off), 8-bit codes
+//     are converted (128 is taken off).
+//   O^T[dim, (row, group)] += V' A^T, A = p step of the column's group as bf16
+//     hi + lo (error below 2^-16: one bf16 would be off by 2^-8 of the group's
+//     half range, whatever the value), and p mid in fp32 beside it; row c of V'
+//     product i is dim (D / 16) c + i of every run, all in group i / 4. The
+//     offset's sum over A is one more product with constant rows.
+// P never leaves its lane: the C layout of S^T (lane: 4 keys of a column) is the
+// B operand of O^T when the 32 keys of a step are taken in the order {4 kg .. 4
+// kg + 3, 16 + 4 kg ..}. Codes are exact.
+//
+// The running maximum m (log2 units) moves only when a tile passes it by 8, so O
+// is rescaled a few times a row. Tiles are dealt in turn, so any valid length
+// spreads over all splits, and a wave's first tile does not depend on it: its
+// loads go out before the length arrives. Keys past a row's end are masked in S
+// and their A and mid set to zero, whatever their params hold.
+template <int D, int BITS, int HP>
+struct KvqFew {
+  static constexpr int NG = D / 64, GT = NG < 16 / HP ? NG : 16 / HP, CT = NG / GT, NW = 4;
+  static constexpr int KW = BITS / 2;                   // words of a lane's 16 dims of a key group
+  static constexpr int VW = D * BITS / 512;             // words of a run (0: 16 bits)
+  static constexpr int VR = VW ? VW : 1;
+  static constexpr int RB = D * BITS / 8;               // bytes of a packed row
+  static constexpr float OFF = BITS == 4 ? 24.f : 128.f, HALF = BITS == 4 ? 8.f : 128.f;
+  static constexpr int REC = HP * (D + 2);              // floats of a split's record
+};
+
+struct KvqArgs {
+  const uint16_t* q;
+  const uint8_t *kq, *vq;
+  const uint32_t *kp, *vp;
+  const long long* len;
+  int n_len;
+  long long offset;
+  const uint16_t* gate;
+  long long gate_stride;
+  float scale;
+  uint16_t* out;
+  float* part;
+  int QH, KVH, L, C, blocks, splits, units;  // units = B * KVH * splits
+};
+
+// Keys that row r (head r % G of token r / G) of sequence b sees.
+Q35_DEV int kvq_limit(const KvqArgs& a, long long start, int r, int G) {
+  const long long n = start + r / G + 1;
+  return (int)(n < 0 ? 0 : n > a.C ? a.C : n);
+}
+Q35_DEV long long kvq_start(const KvqArgs& a, int b) {
+  return (a.len ? a.len[a.n_len > 1 ? b : 0] : 0) + a.offset;
+}
+
+// Two 4-bit codes (nibble i of each half of w) as 16 + code in bf16.
+template <int I>
+Q35_DEV uint32_t kvq_pair4(uint32_t w) {
+  const uint32_t t = I == 0 ? w << 3 : w >> (4 * I - 3);
+  return (t & 0x00780078u) | 0x41804180u;
+}
+// Byte i of two words as bf16.
+template <int I>
+Q35_DEV uint32_t kvq_pair8(uint32_t w0, uint32_t w1) {
+  const float a = (float)((w0 >> (8 * I)) & 255u), b = (float)((w1 >> (8 * I)) & 255u);
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+
+Q35_DEV float kvq_xor16_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+Q35_DEV float kvq_xor16_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Over the 4 lanes of a column.
+Q35_DEV float kvq_col_max(float v) { return half_max(kvq_xor16_max(v)); }
+Q35_DEV float kvq_col_sum(float v) { return half_sum(kvq_xor16_sum(v)); }
+
+Q35_DEV q35_f32x4 mfma16(const q35_u32x4 a, const q35_u32x4 b, q35_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_bf16x8, a), __builtin_bit_cast(q35_bf16x8, b),
+                                                 c, 0, 0, 0);
+}
+
+template <int D, int BITS, int HP>
+__global__ __launch_bounds__(256) void kvq_few(const KvqArgs a) {
+  using F = KvqFew<D, BITS, HP>;
+  constexpr int NG = F::NG, GT = F::GT, CT = F::CT, NW = F::NW, KW = F::KW, VR = F::VR, NT = D / 16;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int c16 = lane & 15, kg = lane >> 4, hr = c16 / GT, gl = c16 % GT;
+  // Blocks of the same keys are 8 workgroups apart (one XCD, one L2) and next
+  // in turn.
+  const int u = (int)(blockIdx.x / (8u * a.blocks)) * 8 + (int)(blockIdx.x % 8u);
+  const int blk = (int)(blockIdx.x / 8u) % a.blocks;
+  const int bh = u / a.splits, split = u % a.splits;
+  if (u >= a.units) return;  // the grid is rounded up to 8 units
+  const int b = bh / a.KVH, kvh = bh % a.KVH;
+  const int G = a.QH / a.KVH, R = G * a.L;
+
+  const uint8_t* K = a.kq + (size_t)bh * a.C * F::RB;
+  const uint8_t* V = a.vq + (size_t)bh * a.C * F::RB;
+  const uint32_t* KP = a.kp + (size_t)bh * NG * a.C;
+  const uint32_t* VP = a.vp + (size_t)bh * NG * a.C;
+
+  struct Tile {
+    uint32_t k[2][NG][KW], v[8][VR];
+    uint4 kp[2][CT], vp[2][CT];
+  };
+  const int last_tile = a.C / 32 - 1;
+  auto load = [&](Tile& t, int tile) {
+    const uint32_t key = 32u * (uint32_t)min(tile, last_tile);
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      const uint8_t* p = K + (key + 16 * tt + c16) * F::RB + 4 * KW * kg;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        if constexpr (KW == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(p + 32 * g);
+          t.k[tt][g][0] = x.x; t.k[tt][g][1] = x.y;
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4*>(p + 64 * g);
+          t.k[tt][g][0] = x.x; t.k[tt][g][1] = x.y; t.k[tt][g][2] = x.z; t.k[tt][g][3] = x.w;
+        }
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+        t.kp[tt][ct] = *reinterpret_cast<const uint4*>(KP + (size_t)(ct * GT + gl) * a.C + key + 16 * tt + 4 * kg);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint8_t* p = V + (key + 16 * (j >> 2) + 4 * kg + (j & 3)) * F::RB + (F::RB / 16) * c16;
+      if constexpr (F::VW == 0) t.v[j][0] = *reinterpret_cast<const uint16_t*>(p);
+      else if constexpr (VR == 1) t.v[j][0] = *reinterpret_cast<const uint32_t*>(p);
+      else if constexpr (VR == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        t.v[j][0] = x.x; t.v[j][1] = x.y;
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        t.v[j][0] = x.x; t.v[j][1] = x.y; t.v[j][2] = x.z; t.v[j][3] = x.w;
+      }
+    }
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+        t.vp[tt][ct] = *reinterpret_cast<const uint4*>(VP + (size_t)(ct * GT + gl) * a.C + key + 16 * tt + 4 * kg);
+  };
+  Tile ta, tb;
+  int tile = split * NW + w;
+  const int stride = a.splits * NW;
+  load(ta, tile);
+
+  const long long start = kvq_start(a, b);
+  const int r = min(blk * HP + hr, R - 1);
+  const int limit = kvq_limit(a, start, r, G);
+  const int least = kvq_limit(a, start, blk * HP, G);
+  const int n_max = kvq_limit(a, start, min(blk * HP + HP, R) - 1, G);
+  const int n_tiles = (n_max + 31) / 32;
+
+  // Q of the lane's row: dims 64 g + 16 kg + 8 s + {i, i + 4} in register i of
+  // step s, zero outside the column's group; the sums over whole groups.
+  q35_u32x4 qf[NG][2];
+  float qs[CT];
+  {
+    const uint16_t* qp = a.q + (((size_t)b * a.QH + kvh * G + r % G) * a.L + r / G) * D + 16 * kg;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      q35_u32x4 own[2];
+      float sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const uint4 x = *reinterpret_cast<const uint4*>(qp + 64 * (ct * GT + gl) + 8 * s);
+        sum += ((bf_lo(x.x) + bf_hi(x.x)) + (bf_lo(x.y) + bf_hi(x.y))) +
+               ((bf_lo(x.z) + bf_hi(x.z)) + (bf_lo(x.w) + bf_hi(x.w)));
+        own[s] = q35_u32x4{__builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
+                           __builtin_amdgcn_perm(x.w, x.y, 0x05040100u), __builtin_amdgcn_perm(x.w, x.y, 0x07060302u)};
+      }
+      qs[ct] = kvq_col_sum(sum);
+#pragma unroll
+      for (int x = 0; x < GT; ++x)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[ct * GT + x][s][e] = gl == x ? own[s][e] : 0u;
+    }
+  }
+  const float c2 = a.scale * 1.4426950408889634f;
+  q35_f32x4 o[NT], cnt[CT];
+  float cs[CT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) o[i] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    cnt[ct] = {0.f, 0.f, 0.f, 0.f};
+    cs[ct] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  const uint32_t offs = BITS == 4 ? 0xc1c0c1c0u : 0xc300c300u;  // bf16 -24, -128
+  const q35_u32x4 ones = {offs, offs, offs, offs};
+
+  auto step = [&](const Tile& t, int key0) {
+    float s[8];
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const float z = -F::OFF * qs[ct];
+        q35_f32x4 acc = {z, z, z, z};
+#pragma unroll
+        for (int x = 0; x < GT; ++x) {
+          const int g = ct * GT + x;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            q35_u32x4 kf;
+            if constexpr (BITS == 4) {
+              const uint32_t kw = t.k[tt][g][h];
+              kf = q35_u32x4{kvq_pair4<0>(kw), kvq_pair4<1>(kw), kvq_pair4<2>(kw), kvq_pair4<3>(kw)};
+            } else {
+              const uint32_t k0 = t.k[tt][g][2 * h], k1 = t.k[tt][g][2 * h + 1];
+              kf = q35_u32x4{kvq_pair8<0>(k0, k1), kvq_pair8<1>(k0, k1), kvq_pair8<2>(k0, k1), kvq_pair8<3>(k0, k1)};
+            }
+            acc = mfma16(kf, qf[g][h], acc);
+          }
+        }
+        const uint32_t pw[4] = {t.kp[tt][ct].x, t.kp[tt][ct].y, t.kp[tt][ct].z, t.kp[tt][ct].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float st = bf_lo(pw[i]);
+          part[i] = fmaf(st, acc[i], fmaf(fmaf(F::HALF, st, bf_hi(pw[i])), qs[ct], part[i]));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = part[i];
+        if constexpr (GT > 1) x += dpp_f<Q35_DPP_QUAD_XOR1>(x);
+        if constexpr (GT > 2) x += dpp_f<Q35_DPP_QUAD_XOR2>(x);
+        s[4 * tt + i] = x * c2;
+      }
+    }
+    float vs[CT][8], vm[CT][8];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        const uint32_t pw[4] = {t.vp[tt][ct].x, t.vp[tt][ct].y, t.vp[tt][ct].z, t.vp[tt][ct].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float st = bf_lo(pw[i]);
+          vs[ct][4 * tt + i] = st;
+          vm[ct][4 * tt + i] = fmaf(F::HALF, st, bf_hi(pw[i]));
+        }
+      }
+    if (key0 + 32 > least) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool in = key0 + 16 * (j >> 2) + 4 * kg + (j & 3) < limit;
+        s[j] = in ? s[j] : -INFINITY;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          vs[ct][j] = in ? vs[ct][j] : 0.f;
+          vm[ct][j] = in ? vm[ct][j] : 0.f;
+        }
+      }
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[j]);
+    mx = kvq_col_max(mx);
+    if (__ballot(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx);
+      const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= corr;
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] *= corr;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        cs[ct] *= corr;
+        cnt[ct][0] *= corr;  // the other rows of cnt are copies, unused
+      }
+      m = mn;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;  // a row without any key so far
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = __builtin_amdgcn_exp2f(s[j] - ms);
+      l += p[j];
+    }
+    q35_u32x4 af[CT], al[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = p[2 * e] * vs[ct][2 * e], y = p[2 * e + 1] * vs[ct][2 * e + 1];
+        af[ct][e] = pack_bf2(x, y);
+        al[ct][e] = pack_bf2(x - bf_lo(af[ct][e]), y - bf_hi(af[ct][e]));
+        cs[ct] = fmaf(p[2 * e], vm[ct][2 * e], cs[ct]);
+        cs[ct] = fmaf(p[2 * e + 1], vm[ct][2 * e + 1], cs[ct]);
+      }
+      cnt[ct] = mfma16(ones, af[ct], cnt[ct]);
+      cnt[ct] = mfma16(ones, al[ct], cnt[ct]);
+    }
+    if constexpr (BITS == 4) {
+#pragma unroll
+      for (int x = 0; x < VR; ++x) {
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          lo[e] = __builtin_amdgcn_perm(t.v[2 * e + 1][x], t.v[2 * e][x], 0x05040100u);
+          hi[e] = __builtin_amdgcn_perm(t.v[2 * e + 1][x], t.v[2 * e][x], 0x07060302u);
+        }
+        auto pv = [&](auto tag, const uint32_t (&h)[4], int i) {
+          constexpr int N = decltype(tag)::value;
+          const q35_u32x4 vf = {kvq_pair4<N>(h[0]), kvq_pair4<N>(h[1]), kvq_pair4<N>(h[2]), kvq_pair4<N>(h[3])};
+          o[i] = mfma16(vf, af[i / 4 / GT], o[i]);
+          o[i] = mfma16(vf, al[i / 4 / GT], o[i]);
+        };
+        pv(std::integral_constant<int, 0>{}, lo, 8 * x); pv(std::integral_constant<int, 1>{}, lo, 8 * x + 1);
+        pv(std::integral_constant<int, 2>{}, lo, 8 * x + 2); pv(std::integral_constant<int, 3>{}, lo, 8 * x + 3);
+        if constexpr (NT > 4) {
+          pv(std::integral_constant<int, 0>{}, hi, 8 * x + 4); pv(std::integral_constant<int, 1>{}, hi, 8 * x + 5);
+          pv(std::integral_constant<int, 2>{}, hi, 8 * x + 6); pv(std::integral_constant<int, 3>{}, hi, 8 * x + 7);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < VR; ++x) {
+        auto pv = [&](auto tag) {
+          constexpr int N = decltype(tag)::value;
+          q35_u32x4 vf;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vf[e] = kvq_pair8<N>(t.v[2 * e][x], t.v[2 * e + 1][x]);
+          const int i = 4 * x + N;
+          o[i] = mfma16(vf, af[i / 4 / GT], o[i]);
+          o[i] = mfma16(vf, al[i / 4 / GT], o[i]);
+        };
+        pv(std::integral_constant<int, 0>{}); pv(std::integral_constant<int, 1>{});
+        pv(std::integral_constant<int, 2>{}); pv(std::integral_constant<int, 3>{});
+      }
+    }
+  };
+  // Two register sets in turn, the next tile requested before the current one
+  // is used.
+  while (tile < n_tiles) {
+    const int next = tile + stride;
+    if (next < n_tiles) load(tb, next);
+    step(ta, 32 * tile);
+    tile = next;
+    if (tile >= n_tiles) break;
+    const int after = tile + stride;
+    if (after < n_tiles) load(ta, after);
+    step(tb, 32 * tile);
+    tile = after;
+  }
+
+  // The waves' sums meet in LDS: row hr, dims (D / 16) (4 kg + e) + 4 g .. + 3
+  // of the lane's groups g.
+  __shared__ float o_s[NW][HP][D], ml_s[NW][HP][2];
+  l = kvq_col_sum(l);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const float add = kvq_col_sum(cs[ct]) + cnt[ct][0];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        v[x] = o[4 * ct * GT + x][e];
+#pragma unroll
+        for (int g = 1; g < GT; ++g) v[x] = gl == g ? o[4 * (ct * GT + g) + x][e] : v[x];
+        v[x] += add;
+      }
+      *reinterpret_cast<float4*>(&o_s[w][hr][NT * (4 * kg + e) + 4 * (ct * GT + gl)]) =
+          make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+  if (kg == 0 && gl == 0) {
+    ml_s[w][hr][0] = m;
+    ml_s[w][hr][1] = l;
+  }
+  __syncthreads();
+  float* rec = a.part + ((size_t)(bh * a.blocks + blk) * a.splits + split) * F::REC;
+  for (int x = threadIdx.x; x < HP * D / 4; x += 256) {
+    const int h = x / (D / 4), d = 4 * (x % (D / 4));
+    float mm = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) mm = fmaxf(mm, ml_s[v][h][0]);
+    const float ms = mm == -INFINITY ? 0.f : mm;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float ll = 0.f;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) {
+      const float f = __builtin_amdgcn_exp2f(ml_s[v][h][0] - ms);  // 0 for a wave without keys
+      const float4 t = *reinterpret_cast<const float4*>(&o_s[v][h][d]);
+      sum.x = fmaf(t.x, f, sum.x); sum.y = fmaf(t.y, f, sum.y);
+      sum.z = fmaf(t.z, f, sum.z); sum.w = fmaf(t.w, f, sum.w);
+      ll = fmaf(ml_s[v][h][1], f, ll);
+    }
+    *reinterpret_cast<float4*>(rec + h * D + d) = sum;
+    if (d == 0) *reinterpret_cast<float2*>(rec + HP * D + 2 * h) = make_float2(mm, ll);
+  }
+}
+
+// Merge of the splits that had keys: o = sum_s o_s 2^(m_s - M) / sum_s l_s
+// 2^(m_s - M), M = max m_s. One workgroup a query row and 64 dims, 16 threads of
+// 4 dims by 16 parts of the splits, so a thread reads at most 16 records.
+constexpr int kKvqSplits = 256;
+template <int D, int HP>
+__global__ __launch_bounds__(256) void kvq_few_merge(const KvqArgs a) {
+  constexpr int NW = 4, REC = HP * (D + 2);
+  const int t = threadIdx.x, d = 64 * (int)blockIdx.y + 4 * (t & 15), part = t >> 4;
+  const int G = a.QH / a.KVH, R = G * a.L;
+  const int bh = blockIdx.x / (unsigned)R, r = blockIdx.x % (unsigned)R;
+  const int b = bh / a.KVH, kvh = bh % a.KVH, blk = r / HP, h = r % HP;
+  const long long start = kvq_start(a, b);
+  const int n_max = kvq_limit(a, start, min(blk * HP + HP, R) - 1, G);
+  const int n = min(a.splits, ((n_max + 31) / 32 + NW - 1) / NW);
+  const float* rec = a.part + (size_t)(bh * a.blocks + blk) * a.splits * REC;
+  __shared__ float f_s[kKvqSplits], red_s[2][4];
+  __shared__ float4 sum_s[16][16];
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (t < n) ml = *reinterpret_cast<const float2*>(rec + (size_t)t * REC + HP * D + 2 * h);
+  const float mw = wave_max(ml.x);
+  if ((t & 63) == 0) red_s[0][t >> 6] = mw;
+  __syncthreads();
+  const float mm = fmaxf(fmaxf(red_s[0][0], red_s[0][1]), fmaxf(red_s[0][2], red_s[0][3]));
+  const float f = __builtin_amdgcn_exp2f(ml.x - (mm == -INFINITY ? 0.f : mm));
+  f_s[t] = f;
+  const float lw = wave_sum(ml.y * f);
+  if ((t & 63) == 0) red_s[1][t >> 6] = lw;
+  __syncthreads();
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = part; s < n; s += 16) {
+    const float4 x = *reinterpret_cast<const float4*>(rec + (size_t)s * REC + h * D + d);
+    const float fs = f_s[s];
+    sum.x = fmaf(x.x, fs, sum.x); sum.y = fmaf(x.y, fs, sum.y);
+    sum.z = fmaf(x.z, fs, sum.z); sum.w = fmaf(x.w, fs, sum.w);
+  }
+  sum_s[part][t & 15] = sum;
+  __syncthreads();
+  if (part) return;
+#pragma unroll
+  for (int v = 1; v < 16; ++v) {
+    const float4 x = sum_s[v][t];
+    sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+  }
+  // a row without keys is zero
+  const float inv = kvq_limit(a, start, r, G) ? 1.0f / ((red_s[1][0] + red_s[1][1]) + (red_s[1][2] + red_s[1][3])) : 0.f;
+  const int head = kvh * G + r % G;
+  float v[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+  if (a.gate) {
+    const uint2 x = *reinterpret_cast<const uint2*>(a.gate + b * a.gate_stride + (2 * head + 1) * D + d);
+    v[0] *= sigmoid_f(bf_lo(x.x)); v[1] *= sigmoid_f(bf_hi(x.x));
+    v[2] *= sigmoid_f(bf_lo(x.y)); v[3] *= sigmoid_f(bf_hi(x.y));
+  }
+  *reinterpret_cast<uint2*>(a.out + (((size_t)b * a.L + r / G) * a.QH + head) * D + d) =
+      make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
+}
+
+// Up to this many query rows of a KV head go to kvq_few.
+constexpr int kKvqFewRows = 64;
+// Rows a block of kvq_few holds: as few columns as the row count needs, as a
+// block's vector work grows with its column tiles.
+int kvq_block_rows(int D, long long rows) {
+  if (D == 64) return 16;
+  if (D == 128) return rows <= 8 ? 8 : 16;
+  return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+}
+// Splits of every KV head's keys: from the capacity, as the valid length is not
+// known here; up to kKvqTarget workgroups in all.
+constexpr int kKvqTarget = 512;
+int kvq_splits(int B, int KVH, int blocks, int C) {
+  const long long pieces = (C + 127) / 128;
+  long long s = kKvqTarget / ((long long)B * KVH * blocks);
+  s = s < 1 ? 1 : s > kKvqSplits ? kKvqSplits : s;
+  return (int)(s < pieces ? s : pieces);
+}
+
 bool kvq_shape_ok(int B, int KVH, int L, int D, int bits, int C) {
   return B >= 0 && KVH > 0 && L >= 0 && (D == 64 || D == 128 || D == 256) && (bits == 4 || bits == 8) && C > 0 &&
          C % 32 == 0 && (long long)C * D * bits / 8 < (1ll << 31);
@@ -342,7 +836,10 @@ int q35_kv_dequantize(const void* kq, const void* vq, const void* kp, const void
 
 long long q35_gqa_attention_kvq_workspace(int B, int QH, int KVH, int L, int D, int bits, int capacity) {
   if (!kvq_shape_ok(B, KVH, L, D, bits, capacity) || QH <= 0 || QH % KVH) return -1;
-  return 0;
+  const long long rows = (long long)(QH / KVH) * L;
+  if ((long long)B * L == 0 || rows > kKvqFewRows) return 0;
+  const int hp = kvq_block_rows(D, rows), blocks = (int)((rows + hp - 1) / hp);
+  return (long long)B * KVH * blocks * kvq_splits(B, KVH, blocks, capacity) * hp * (D + 2);
 }
 
 int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const void* kp, const void* vp,
@@ -355,14 +852,41 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
   Q35_CHECK_ARG(!gate || L == 1);
   Q35_CHECK_ARG(q && kq && vq && kp && vp && out && q35_aligned16(kq) && q35_aligned16(vq) && q35_aligned16(kp) &&
                 q35_aligned16(vp) && q35_aligned16(q) && q35_aligned16(out) && q35_aligned8(gate));
-  const long long rows = (long long)B * QH * L;
-  Q35_CHECK_ARG(rows < (1ll << 31));
-  const unsigned grid = (unsigned)((rows + 3) / 4);
+  const long long rows = (long long)(QH / KVH) * L;
+  Q35_CHECK_ARG((long long)B * KVH * rows < (1ll << 31));
+  if (rows <= kKvqFewRows) {
+    const int hp = kvq_block_rows(D, rows), blocks = (int)((rows + hp - 1) / hp);
+    const int splits = kvq_splits(B, KVH, blocks, capacity);
+    const long long units = (long long)B * KVH * splits;
+    Q35_CHECK_ARG(workspace && q35_aligned16(workspace) &&
+                  workspace_floats >= units * blocks * hp * (D + 2) && (units + 7) * blocks < (1ll << 31));
+    const KvqArgs a{(const uint16_t*)q, (const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,
+                    (const uint32_t*)vp, (const long long*)len_dev, n_len, offset, (const uint16_t*)gate, gate_stride,
+                    scale, (uint16_t*)out, (float*)workspace, QH, KVH, L, capacity, blocks, splits, (int)units};
+    const unsigned grid = (unsigned)((units + 7) / 8 * 8 * blocks);
+    const dim3 mgrid((unsigned)(B * KVH * rows), (unsigned)(D / 64));
+#define Q35_FEW(DD, HP)                                             \
+  do {                                                              \
+    if (bits == 4) kvq_few<DD, 4, HP><<<grid, 256, 0, stream>>>(a); \
+    else kvq_few<DD, 8, HP><<<grid, 256, 0, stream>>>(a);           \
+    kvq_few_merge<DD, HP><<<mgrid, 256, 0, stream>>>(a);            \
+  } while (0)
+    if (D == 64) Q35_FEW(64, 16);
+    else if (D == 128 && hp == 8) Q35_FEW(128, 8);
+    else if (D == 128) Q35_FEW(128, 16);
+    else if (hp == 4) Q35_FEW(256, 4);
+    else if (hp == 8) Q35_FEW(256, 8);
+    else Q35_FEW(256, 16);
+#undef Q35_FEW
+    return q35_last_error();
+  }
+  const long long waves = (long long)B * QH * L;
+  const unsigned grid = (unsigned)((waves + 3) / 4);
 #define Q35_CALL(E, BITS)                                                                                           \
   kvq_attend_rows<E / 4, BITS><<<grid, 256, 0, stream>>>(                                                           \
       (const uint16_t*)q, (const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp, (const uint32_t*)vp,          \
       (const long long*)len_dev, n_len, offset, (const uint16_t*)gate, gate_stride, scale, (uint16_t*)out, QH, KVH,  \
-      L, capacity, rows)
+      L, capacity, waves)
   Q35_KVQ_BY_D(Q35_CALL);
 #undef Q35_CALL
   return q35_last_error();
