@@ -308,6 +308,26 @@ __global__ __launch_bounds__(256) void kvq_attend_rows(
 // spreads over all splits, and a wave's first tile does not depend on it: its
 // loads go out before the length arrives. Keys past a row's end are masked in S
 // and their A and mid set to zero, whatever their params hold.
+typedef uint32_t q35_u32x2 __attribute__((ext_vector_type(2)));
+Q35_DEV __amdgpu_buffer_rsrc_t kvq_buffer(const void* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
+}
+// W words (0: 16 bits) at byte at + tile.
+template <int W>
+Q35_DEV void kvq_load(uint32_t* d, __amdgpu_buffer_rsrc_t r, uint32_t at, uint32_t tile) {
+  if constexpr (W == 0) {
+    d[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at, tile, 0);
+  } else if constexpr (W == 1) {
+    d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, tile, 0);
+  } else if constexpr (W == 2) {
+    const q35_u32x2 x = __builtin_bit_cast(q35_u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, at, tile, 0));
+    d[0] = x.x; d[1] = x.y;
+  } else {
+    const q35_u32x4 x = __builtin_bit_cast(q35_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, tile, 0));
+    d[0] = x.x; d[1] = x.y; d[2] = x.z; d[3] = x.w;
+  }
+}
+
 template <int D, int BITS, int HP>
 struct KvqFew {
   static constexpr int NG = D / 64, GT = NG < 16 / HP ? NG : 16 / HP, CT = NG / GT, NW = 4;
@@ -317,6 +337,11 @@ struct KvqFew {
   static constexpr int RB = D * BITS / 8;               // bytes of a packed row
   static constexpr float OFF = BITS == 4 ? 24.f : 128.f, HALF = BITS == 4 ? 8.f : 128.f;
   static constexpr int REC = HP * (D + 2);              // floats of a split's record
+  struct Tile {  // a wave's 32 keys in flight
+    uint32_t k[2][NG][KW], v[8][VR];
+    uint32_t kp[2][CT][4], vp[2][CT][4];
+  };
+  static constexpr int WAVES = BITS == 4 && !(D == 256 && HP > 4) ? 2 : 1;  // waves a SIMD, by registers
 };
 
 struct KvqArgs {
@@ -344,10 +369,19 @@ Q35_DEV long long kvq_start(const KvqArgs& a, int b) {
 }
 
 // Two 4-bit codes (nibble i of each half of w) as 16 + code in bf16.
+// One v_and_or_b32 takes its constants from registers, one of them a vector's.
+struct KvqMask {
+  uint32_t mask, off;
+};
+Q35_DEV KvqMask kvq_mask() {
+  KvqMask c{0x00780078u, 0x41804180u};
+  asm("" : "+s"(c.mask), "+v"(c.off));
+  return c;
+}
 template <int I>
-Q35_DEV uint32_t kvq_pair4(uint32_t w) {
+Q35_DEV uint32_t kvq_pair4(uint32_t w, const KvqMask& c) {
   const uint32_t t = I == 0 ? w << 3 : w >> (4 * I - 3);
-  return (t & 0x00780078u) | 0x41804180u;
+  return (t & c.mask) | c.off;
 }
 // Byte i of two words as bf16.
 template <int I>
@@ -374,7 +408,7 @@ Q35_DEV q35_f32x4 mfma16(const q35_u32x4 a, const q35_u32x4 b, q35_f32x4 c) {
 }
 
 template <int D, int BITS, int HP>
-__global__ __launch_bounds__(256) void kvq_few(const KvqArgs a) {
+__global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(const KvqArgs a) {
   using F = KvqFew<D, BITS, HP>;
   constexpr int NG = F::NG, GT = F::GT, CT = F::CT, NW = F::NW, KW = F::KW, VR = F::VR, NT = D / 16;
   const int lane = threadIdx.x & 63;
@@ -394,48 +428,35 @@ __global__ __launch_bounds__(256) void kvq_few(const KvqArgs a) {
   const uint32_t* KP = a.kp + (size_t)bh * NG * a.C;
   const uint32_t* VP = a.vp + (size_t)bh * NG * a.C;
 
-  struct Tile {
-    uint32_t k[2][NG][KW], v[8][VR];
-    uint4 kp[2][CT], vp[2][CT];
-  };
+  using Tile = typename F::Tile;
+  // Buffer loads: the head's arrays as resources, a tile's place as the scalar
+  // offset, a lane's place in it constant, so no 64-bit vector address lives in
+  // the loop. (A head's codes stay below 2 GiB.)
   const int last_tile = a.C / 32 - 1;
+  const auto kr = kvq_buffer(K, (uint32_t)a.C * F::RB), vr = kvq_buffer(V, (uint32_t)a.C * F::RB);
+  const auto kpr = kvq_buffer(KP, 4u * NG * (uint32_t)a.C), vpr = kvq_buffer(VP, 4u * NG * (uint32_t)a.C);
+  uint32_t k_at = (uint32_t)c16 * F::RB + 4 * KW * kg, v_at = 4u * kg * F::RB + (F::RB / 16) * c16;
+  uint32_t p_at = 4u * ((uint32_t)gl * a.C + 4 * kg);
+  const uint32_t p_ct = 4u * GT * (uint32_t)a.C;
   auto load = [&](Tile& t, int tile) {
+    // what is added to these stays in the instructions, not in registers
+    asm volatile("" : "+v"(k_at), "+v"(v_at), "+v"(p_at));
     const uint32_t key = 32u * (uint32_t)min(tile, last_tile);
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      const uint8_t* p = K + (key + 16 * tt + c16) * F::RB + 4 * KW * kg;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        if constexpr (KW == 2) {
-          const uint2 x = *reinterpret_cast<const uint2*>(p + 32 * g);
-          t.k[tt][g][0] = x.x; t.k[tt][g][1] = x.y;
-        } else {
-          const uint4 x = *reinterpret_cast<const uint4*>(p + 64 * g);
-          t.k[tt][g][0] = x.x; t.k[tt][g][1] = x.y; t.k[tt][g][2] = x.z; t.k[tt][g][3] = x.w;
-        }
-      }
+      for (int g = 0; g < NG; ++g)
+        kvq_load<KW>(t.k[tt][g], kr, k_at + (16 * F::RB * tt + 16 * KW * g), key * F::RB);
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-        t.kp[tt][ct] = *reinterpret_cast<const uint4*>(KP + (size_t)(ct * GT + gl) * a.C + key + 16 * tt + 4 * kg);
+      for (int ct = 0; ct < CT; ++ct) kvq_load<4>(t.kp[tt][ct], kpr, p_at + p_ct * ct + 64 * tt, 4 * key);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint8_t* p = V + (key + 16 * (j >> 2) + 4 * kg + (j & 3)) * F::RB + (F::RB / 16) * c16;
-      if constexpr (F::VW == 0) t.v[j][0] = *reinterpret_cast<const uint16_t*>(p);
-      else if constexpr (VR == 1) t.v[j][0] = *reinterpret_cast<const uint32_t*>(p);
-      else if constexpr (VR == 2) {
-        const uint2 x = *reinterpret_cast<const uint2*>(p);
-        t.v[j][0] = x.x; t.v[j][1] = x.y;
-      } else {
-        const uint4 x = *reinterpret_cast<const uint4*>(p);
-        t.v[j][0] = x.x; t.v[j][1] = x.y; t.v[j][2] = x.z; t.v[j][3] = x.w;
-      }
-    }
+    for (int j = 0; j < 8; ++j)
+      kvq_load<F::VW>(t.v[j], vr, v_at + (16 * (j >> 2) + (j & 3)) * F::RB, key * F::RB);
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-        t.vp[tt][ct] = *reinterpret_cast<const uint4*>(VP + (size_t)(ct * GT + gl) * a.C + key + 16 * tt + 4 * kg);
+      for (int ct = 0; ct < CT; ++ct) kvq_load<4>(t.vp[tt][ct], vpr, p_at + p_ct * ct + 64 * tt, 4 * key);
   };
   Tile ta, tb;
   int tile = split * NW + w;
@@ -449,9 +470,10 @@ __global__ __launch_bounds__(256) void kvq_few(const KvqArgs a) {
   const int n_max = kvq_limit(a, start, min(blk * HP + HP, R) - 1, G);
   const int n_tiles = (n_max + 31) / 32;
 
-  // Q of the lane's row: dims 64 g + 16 kg + 8 s + {i, i + 4} in register i of
-  // step s, zero outside the column's group; the sums over whole groups.
-  q35_u32x4 qf[NG][2];
+  // Q of the lane's row: dims 64 g + 16 kg + 8 s + {i, i + 4} in word i of step
+  // s, zero outside the column's group; the sums over whole groups. The four
+  // waves need the same operands, which stay in LDS to save registers.
+  __shared__ q35_u32x4 q_s[NG][2][64];
   float qs[CT];
   {
     const uint16_t* qp = a.q + (((size_t)b * a.QH + kvh * G + r % G) * a.L + r / G) * D + 16 * kg;
@@ -472,11 +494,12 @@ __global__ __launch_bounds__(256) void kvq_few(const KvqArgs a) {
       for (int x = 0; x < GT; ++x)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qf[ct * GT + x][s][e] = gl == x ? own[s][e] : 0u;
+          if (w == (2 * (ct * GT + x) + s) % NW) q_s[ct * GT + x][s][lane] = gl == x ? own[s] : q35_u32x4{0, 0, 0, 0};
     }
   }
+  lds_barrier();
   const float c2 = a.scale * 1.4426950408889634f;
+  const KvqMask cm = kvq_mask();
   q35_f32x4 o[NT], cnt[CT];
   float cs[CT];
 #pragma unroll
@@ -491,6 +514,7 @@ __global__ __launch_bounds__(256) void kvq_few(const KvqArgs a) {
   const q35_u32x4 ones = {offs, offs, offs, offs};
 
   auto step = [&](const Tile& t, int key0) {
+    asm volatile("" : : : "memory");  // keeps Q's reads in the loop: hoisted, they take the registers again
     float s[8];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
@@ -507,15 +531,15 @@ __global__ __launch_bounds__(256) void kvq_few(const KvqArgs a) {
             q35_u32x4 kf;
             if constexpr (BITS == 4) {
               const uint32_t kw = t.k[tt][g][h];
-              kf = q35_u32x4{kvq_pair4<0>(kw), kvq_pair4<1>(kw), kvq_pair4<2>(kw), kvq_pair4<3>(kw)};
+              kf = q35_u32x4{kvq_pair4<0>(kw, cm), kvq_pair4<1>(kw, cm), kvq_pair4<2>(kw, cm), kvq_pair4<3>(kw, cm)};
             } else {
               const uint32_t k0 = t.k[tt][g][2 * h], k1 = t.k[tt][g][2 * h + 1];
               kf = q35_u32x4{kvq_pair8<0>(k0, k1), kvq_pair8<1>(k0, k1), kvq_pair8<2>(k0, k1), kvq_pair8<3>(k0, k1)};
             }
-            acc = mfma16(kf, qf[g][h], acc);
+            acc = mfma16(kf, q_s[g][h][lane], acc);
           }
         }
-        const uint32_t pw[4] = {t.kp[tt][ct].x, t.kp[tt][ct].y, t.kp[tt][ct].z, t.kp[tt][ct].w};
+        const uint32_t(&pw)[4] = t.kp[tt][ct];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float st = bf_lo(pw[i]);
@@ -535,7 +559,7 @@ __global__ __launch_bounds__(256) void kvq_few(const KvqArgs a) {
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
-        const uint32_t pw[4] = {t.vp[tt][ct].x, t.vp[tt][ct].y, t.vp[tt][ct].z, t.vp[tt][ct].w};
+        const uint32_t(&pw)[4] = t.vp[tt][ct];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float st = bf_lo(pw[i]);
@@ -606,7 +630,7 @@ __global__ __launch_bounds__(256) void kvq_few(const KvqArgs a) {
         }
         auto pv = [&](auto tag, const uint32_t (&h)[4], int i) {
           constexpr int N = decltype(tag)::value;
-          const q35_u32x4 vf = {kvq_pair4<N>(h[0]), kvq_pair4<N>(h[1]), kvq_pair4<N>(h[2]), kvq_pair4<N>(h[3])};
+          const q35_u32x4 vf = {kvq_pair4<N>(h[0], cm), kvq_pair4<N>(h[1], cm), kvq_pair4<N>(h[2], cm), kvq_pair4<N>(h[3], cm)};
           o[i] = mfma16(vf, af[i / 4 / GT], o[i]);
           o[i] = mfma16(vf, al[i / 4 / GT], o[i]);
         };
@@ -635,17 +659,20 @@ __global__ __launch_bounds__(256) void kvq_few(const KvqArgs a) {
     }
   };
   // Two register sets in turn, the next tile requested before the current one
-  // is used.
+  // is used; always a request (past the end for the current tile again), as with
+  // a branch around it the wait for a tile becomes one for its successor too.
   while (tile < n_tiles) {
     const int next = tile + stride;
-    if (next < n_tiles) load(tb, next);
+    load(tb, next < n_tiles ? next : tile);
+    Q35_PIN();  // the tile's first use waits; its successor's requests go first
     step(ta, 32 * tile);
-    tile = next;
-    if (tile >= n_tiles) break;
-    const int after = tile + stride;
-    if (after < n_tiles) load(ta, after);
-    step(tb, 32 * tile);
-    tile = after;
+    if (next >= n_tiles) break;
+    tile = next + stride;
+    Q35_PIN();
+    load(ta, tile < n_tiles ? tile : next);
+    Q35_PIN();
+    step(tb, 32 * next);
+    Q35_PIN();
   }
 
   // The waves' sums meet in LDS: row hr, dims (D / 16) (4 kg + e) + 4 g .. + 3
