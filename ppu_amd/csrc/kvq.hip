@@ -308,40 +308,24 @@ __global__ __launch_bounds__(256) void kvq_attend_rows(
 // spreads over all splits, and a wave's first tile does not depend on it: its
 // loads go out before the length arrives. Keys past a row's end are masked in S
 // and their A and mid set to zero, whatever their params hold.
-typedef uint32_t q35_u32x2 __attribute__((ext_vector_type(2)));
-Q35_DEV __amdgpu_buffer_rsrc_t kvq_buffer(const void* p, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
-}
-// W words (0: 16 bits) at byte at + tile.
-template <int W>
-Q35_DEV void kvq_load(uint32_t* d, __amdgpu_buffer_rsrc_t r, uint32_t at, uint32_t tile) {
-  if constexpr (W == 0) {
-    d[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at, tile, 0);
-  } else if constexpr (W == 1) {
-    d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, tile, 0);
-  } else if constexpr (W == 2) {
-    const q35_u32x2 x = __builtin_bit_cast(q35_u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, at, tile, 0));
-    d[0] = x.x; d[1] = x.y;
-  } else {
-    const q35_u32x4 x = __builtin_bit_cast(q35_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, tile, 0));
-    d[0] = x.x; d[1] = x.y; d[2] = x.z; d[3] = x.w;
-  }
-}
-
 template <int D, int BITS, int HP>
 struct KvqFew {
   static constexpr int NG = D / 64, GT = NG < 16 / HP ? NG : 16 / HP, CT = NG / GT, NW = 4;
   static constexpr int KW = BITS / 2;                   // words of a lane's 16 dims of a key group
-  static constexpr int VW = D * BITS / 512;             // words of a run (0: 16 bits)
-  static constexpr int VR = VW ? VW : 1;
   static constexpr int RB = D * BITS / 8;               // bytes of a packed row
+  static constexpr int RUN = RB / 16;                   // bytes of a run
+  static constexpr int VR = RUN < 4 ? 1 : RUN / 4;      // words that hold it
+  static constexpr int NK = RB / 32;                    // 1 KiB copies of a tile's keys (and of its values)
+  static constexpr int NI = 2 * NK + 1;                 // copies of a tile
+  static constexpr int STAGE = 1024 * NI;               // keys, values, params (2 NG lines of 128 bytes)
+  static constexpr int RING = 2 * STAGE;                // a wave's two tiles
+  static constexpr int QB = HP * D * 2;                 // bytes of a block's queries
   static constexpr float OFF = BITS == 4 ? 24.f : 128.f, HALF = BITS == 4 ? 8.f : 128.f;
   static constexpr int REC = HP * (D + 2);              // floats of a split's record
-  struct Tile {  // a wave's 32 keys in flight
-    uint32_t k[2][NG][KW], v[8][VR];
-    uint32_t kp[2][CT][4], vp[2][CT][4];
-  };
   static constexpr int WAVES = BITS == 4 && !(D == 256 && HP > 4) ? 2 : 1;  // waves a SIMD, by registers
+  struct Tile {
+    uint32_t k[2][NG][KW], v[8][VR], kp[2][CT][4], vp[2][CT][4];
+  };
 };
 
 struct KvqArgs {
@@ -367,6 +351,16 @@ Q35_DEV int kvq_limit(const KvqArgs& a, long long start, int r, int G) {
 Q35_DEV long long kvq_start(const KvqArgs& a, int b) {
   return (a.len ? a.len[a.n_len > 1 ? b : 0] : 0) + a.offset;
 }
+
+// One wave instruction of a copy: lane i's 16 bytes at p to LDS bytes [lds + 16
+// i, +16).
+Q35_DEV void kvq_copy(uint32_t lds, const uint8_t* p) {
+  asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(lds) : "memory");
+}
+// The slot of chunk 0 of a key row of RB bytes in LDS; the place of value row r.
+template <int RB>
+Q35_DEV uint32_t kvq_swz(uint32_t row) { return row / (256 / RB) % (RB / 16); }
+Q35_DEV uint32_t kvq_turn(uint32_t r) { return (r & 16) | ((r & 3) << 2) | ((r >> 2) & 3); }
 
 // Two 4-bit codes (nibble i of each half of w) as 16 + code in bf16.
 // One v_and_or_b32 takes its constants from registers, one of them a vector's.
@@ -410,6 +404,7 @@ Q35_DEV q35_f32x4 mfma16(const q35_u32x4 a, const q35_u32x4 b, q35_f32x4 c) {
 template <int D, int BITS, int HP>
 __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(const KvqArgs a) {
   using F = KvqFew<D, BITS, HP>;
+  using Tile = typename F::Tile;
   constexpr int NG = F::NG, GT = F::GT, CT = F::CT, NW = F::NW, KW = F::KW, VR = F::VR, NT = D / 16;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -423,67 +418,128 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   const int b = bh / a.KVH, kvh = bh % a.KVH;
   const int G = a.QH / a.KVH, R = G * a.L;
 
-  const uint8_t* K = a.kq + (size_t)bh * a.C * F::RB;
-  const uint8_t* V = a.vq + (size_t)bh * a.C * F::RB;
-  const uint32_t* KP = a.kp + (size_t)bh * NG * a.C;
-  const uint32_t* VP = a.vp + (size_t)bh * NG * a.C;
+  __shared__ alignas(1024) uint8_t lds[NW * F::RING + F::QB];
+  __shared__ float ml_s[NW][HP][2];
+  uint8_t* ring = lds + w * F::RING;
+  uint8_t* q_raw = lds + NW * F::RING;
+  const uint32_t ring0 = __builtin_amdgcn_readfirstlane(lds_offset(ring));
 
-  using Tile = typename F::Tile;
-  // Buffer loads: the head's arrays as resources, a tile's place as the scalar
-  // offset, a lane's place in it constant, so no 64-bit vector address lives in
-  // the loop. (A head's codes stay below 2 GiB.)
-  const int last_tile = a.C / 32 - 1;
-  const auto kr = kvq_buffer(K, (uint32_t)a.C * F::RB), vr = kvq_buffer(V, (uint32_t)a.C * F::RB);
-  const auto kpr = kvq_buffer(KP, 4u * NG * (uint32_t)a.C), vpr = kvq_buffer(VP, 4u * NG * (uint32_t)a.C);
-  uint32_t k_at = (uint32_t)c16 * F::RB + 4 * KW * kg, v_at = 4u * kg * F::RB + (F::RB / 16) * c16;
-  uint32_t p_at = 4u * ((uint32_t)gl * a.C + 4 * kg);
-  const uint32_t p_ct = 4u * GT * (uint32_t)a.C;
-  auto load = [&](Tile& t, int tile) {
-    // what is added to these stays in the instructions, not in registers
-    asm volatile("" : "+v"(k_at), "+v"(v_at), "+v"(p_at));
-    const uint32_t key = 32u * (uint32_t)min(tile, last_tile);
+  // ---- queries of the block into LDS, wave w's share 1 KiB at a time
+  const long long start = kvq_start(a, b);
+  const int row0 = blk * HP;
+#pragma unroll
+  for (int z = 0; z < (F::QB + 1024 * NW - 1) / (1024 * NW); ++z) {
+    const int at = 1024 * (w + NW * z);
+    if (at < F::QB) {
+      const int r = min(row0 + (at + 16 * lane) / (2 * D), R - 1);
+      kvq_copy(__builtin_amdgcn_readfirstlane(lds_offset(q_raw + at)),
+               (const uint8_t*)(a.q + (((size_t)b * a.QH + kvh * G + r % G) * a.L + r / G) * D) +
+                   (at + 16 * lane) % (2 * D));
+    }
+  }
+
+  // ---- a tile: every copy takes 1 KiB in whole rows. Key rows keep their
+  // order, chunk c of 16 bytes at slot c ^ swz(row), so the 16 rows of a
+  // fragment read fall on distinct bank groups; value rows sit transposed, 4 x
+  // 4 within 16, so the 4 rows of a read do.
+  constexpr int RB = F::RB, CPR = RB / 16;
+  const uint8_t* K = a.kq + (size_t)bh * a.C * RB;
+  const uint8_t* V = a.vq + (size_t)bh * a.C * RB;
+  uint32_t k_at[F::NK], v_at[F::NK];
+#pragma unroll
+  for (int z = 0; z < F::NK; ++z) {
+    const uint32_t row = (64 * z + lane) / CPR, slot = lane % CPR;
+    k_at[z] = row * RB + 16 * (slot ^ kvq_swz<RB>(row));
+    v_at[z] = kvq_turn(row) * RB + 16 * slot;
+  }
+  const uint8_t* p_at;
+  {
+    const int i = lane % (16 * NG), g = i / 8 % NG;
+    p_at = (const uint8_t*)((i < 8 * NG ? a.kp : a.vp) + ((size_t)bh * NG + g) * a.C) + 16 * (i % 8);
+  }
+  auto issue = [&](int tile, int stage) {
+    const uint32_t to = ring0 + F::STAGE * stage;
+    const uint8_t *kb = K + (size_t)tile * (32 * RB), *vb = V + (size_t)tile * (32 * RB);
+#pragma unroll
+    for (int z = 0; z < F::NK; ++z) dma16(to + 1024 * z, kb, k_at[z]);
+    kvq_copy(to + 2048 * F::NK, p_at + (size_t)tile * 128);
+#pragma unroll
+    for (int z = 0; z < F::NK; ++z) dma16(to + 1024 * (F::NK + z), vb, v_at[z]);
+  };
+  const int r = min(row0 + hr, R - 1);
+  const int limit = kvq_limit(a, start, r, G);
+  const int least = kvq_limit(a, start, row0, G);
+  const int n_max = kvq_limit(a, start, min(row0 + HP, R) - 1, G);
+  const int n_tiles = (n_max + 31) / 32;
+  const int stride = a.splits * NW;
+  int tile = split * NW + w;
+  if (tile < n_tiles) issue(tile, 0);
+  if (tile + stride < n_tiles) issue(tile + stride, 1);
+
+  // ---- fragment addresses in a stage
+  uint32_t k_rd[2], v_rd, p_rd;
+#pragma unroll
+  for (int tt = 0; tt < 2; ++tt) k_rd[tt] = (16 * tt + c16) * RB;
+  v_rd = 1024 * F::NK + kg * RB + F::RUN * c16;  // token 16 tt + 4 kg + j at row 16 tt + 4 j + kg
+  p_rd = 2048 * F::NK + 128 * gl + 16 * kg;
+  auto fetch = [&](Tile& t, int stage) {
+    const uint8_t* s = ring + F::STAGE * stage;
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
-        kvq_load<KW>(t.k[tt][g], kr, k_at + (16 * F::RB * tt + 16 * KW * g), key * F::RB);
+      for (int g = 0; g < NG; ++g) {
+        // the lane's 16 dims: bytes 4 KW (4 g + kg)
+        const uint32_t c = KW == 4 ? 4 * g + kg : 2 * g + (kg >> 1);
+        const uint8_t* p = s + k_rd[tt] + 16 * (c ^ kvq_swz<RB>(16 * tt + c16)) + (KW == 4 ? 0 : 8 * (kg & 1));
+        if constexpr (KW == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(p);
+          t.k[tt][g][0] = x.x; t.k[tt][g][1] = x.y;
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4*>(p);
+          t.k[tt][g][0] = x.x; t.k[tt][g][1] = x.y; t.k[tt][g][2] = x.z; t.k[tt][g][3] = x.w;
+        }
+      }
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) kvq_load<4>(t.kp[tt][ct], kpr, p_at + p_ct * ct + 64 * tt, 4 * key);
+      for (int ct = 0; ct < CT; ++ct) {
+        const uint4 x = *reinterpret_cast<const uint4*>(s + p_rd + 128 * GT * ct + 64 * tt);
+        t.kp[tt][ct][0] = x.x; t.kp[tt][ct][1] = x.y; t.kp[tt][ct][2] = x.z; t.kp[tt][ct][3] = x.w;
+        const uint4 y = *reinterpret_cast<const uint4*>(s + p_rd + 128 * (NG + GT * ct) + 64 * tt);
+        t.vp[tt][ct][0] = y.x; t.vp[tt][ct][1] = y.y; t.vp[tt][ct][2] = y.z; t.vp[tt][ct][3] = y.w;
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      kvq_load<F::VW>(t.v[j], vr, v_at + (16 * (j >> 2) + (j & 3)) * F::RB, key * F::RB);
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) kvq_load<4>(t.vp[tt][ct], vpr, p_at + p_ct * ct + 64 * tt, 4 * key);
+    for (int j = 0; j < 8; ++j) {
+      const uint8_t* p = s + v_rd + (16 * (j >> 2) + 4 * (j & 3)) * RB;
+      if constexpr (F::RUN == 2) t.v[j][0] = *reinterpret_cast<const uint16_t*>(p);
+      else if constexpr (F::RUN == 4) t.v[j][0] = *reinterpret_cast<const uint32_t*>(p);
+      else if constexpr (F::RUN == 8) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        t.v[j][0] = x.x; t.v[j][1] = x.y;
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        t.v[j][0] = x.x; t.v[j][1] = x.y; t.v[j][2] = x.z; t.v[j][3] = x.w;
+      }
+    }
   };
-  Tile ta, tb;
-  int tile = split * NW + w;
-  const int stride = a.splits * NW;
-  load(ta, tile);
 
-  const long long start = kvq_start(a, b);
-  const int r = min(blk * HP + hr, R - 1);
-  const int limit = kvq_limit(a, start, r, G);
-  const int least = kvq_limit(a, start, blk * HP, G);
-  const int n_max = kvq_limit(a, start, min(blk * HP + HP, R) - 1, G);
-  const int n_tiles = (n_max + 31) / 32;
-
-  // Q of the lane's row: dims 64 g + 16 kg + 8 s + {i, i + 4} in word i of step
-  // s, zero outside the column's group; the sums over whole groups. The four
-  // waves need the same operands, which stay in LDS to save registers.
-  __shared__ q35_u32x4 q_s[NG][2][64];
+  // ---- Q of the lane's row: dims 64 g + 16 kg + 8 s + {i, i + 4} in word i of
+  // step s, zero outside the column's group; the sums over whole groups. The
+  // queries were copied first: they are there when at most the tiles are not.
+  if (tile + stride < n_tiles) wait_vm<2 * F::NI>();
+  else if (tile < n_tiles) wait_vm<F::NI>();
+  else wait_vm<0>();
+  __syncthreads();
+  q35_u32x4 qf[NG][2];
   float qs[CT];
   {
-    const uint16_t* qp = a.q + (((size_t)b * a.QH + kvh * G + r % G) * a.L + r / G) * D + 16 * kg;
+    const uint8_t* qp = q_raw + hr * (2 * D) + 32 * kg;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       q35_u32x4 own[2];
       float sum = 0.f;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const uint4 x = *reinterpret_cast<const uint4*>(qp + 64 * (ct * GT + gl) + 8 * s);
+        const uint4 x = *reinterpret_cast<const uint4*>(qp + 128 * (ct * GT + gl) + 16 * s);
         sum += ((bf_lo(x.x) + bf_hi(x.x)) + (bf_lo(x.y) + bf_hi(x.y))) +
                ((bf_lo(x.z) + bf_hi(x.z)) + (bf_lo(x.w) + bf_hi(x.w)));
         own[s] = q35_u32x4{__builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
@@ -494,10 +550,10 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
       for (int x = 0; x < GT; ++x)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
-          if (w == (2 * (ct * GT + x) + s) % NW) q_s[ct * GT + x][s][lane] = gl == x ? own[s] : q35_u32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[ct * GT + x][s][e] = gl == x ? own[s][e] : 0u;
     }
   }
-  lds_barrier();
   const float c2 = a.scale * 1.4426950408889634f;
   const KvqMask cm = kvq_mask();
   q35_f32x4 o[NT], cnt[CT];
@@ -514,7 +570,6 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   const q35_u32x4 ones = {offs, offs, offs, offs};
 
   auto step = [&](const Tile& t, int key0) {
-    asm volatile("" : : : "memory");  // keeps Q's reads in the loop: hoisted, they take the registers again
     float s[8];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
@@ -536,7 +591,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
               const uint32_t k0 = t.k[tt][g][2 * h], k1 = t.k[tt][g][2 * h + 1];
               kf = q35_u32x4{kvq_pair8<0>(k0, k1), kvq_pair8<1>(k0, k1), kvq_pair8<2>(k0, k1), kvq_pair8<3>(k0, k1)};
             }
-            acc = mfma16(kf, q_s[g][h][lane], acc);
+            acc = mfma16(kf, qf[g][h], acc);
           }
         }
         const uint32_t(&pw)[4] = t.kp[tt][ct];
@@ -658,26 +713,27 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
       }
     }
   };
-  // Two register sets in turn, the next tile requested before the current one
-  // is used; always a request (past the end for the current tile again), as with
-  // a branch around it the wait for a tile becomes one for its successor too.
-  while (tile < n_tiles) {
-    const int next = tile + stride;
-    load(tb, next < n_tiles ? next : tile);
-    Q35_PIN();  // the tile's first use waits; its successor's requests go first
-    step(ta, 32 * tile);
-    if (next >= n_tiles) break;
-    tile = next + stride;
+  // Two tiles in flight: a tile is read into registers whole, then its place
+  // takes the copies of the tile after next, then it is used.
+  for (int stage = 0; tile < n_tiles; stage ^= 1) {
+    if (tile + stride < n_tiles) wait_vm<F::NI>();
+    else wait_vm<0>();
+    asm volatile("" : : : "memory");
     Q35_PIN();
-    load(ta, tile < n_tiles ? tile : next);
+    Tile t;
+    fetch(t, stage);
+    wait_lds();
     Q35_PIN();
-    step(tb, 32 * next);
+    if (tile + 2 * stride < n_tiles) issue(tile + 2 * stride, stage);
     Q35_PIN();
+    step(t, 32 * tile);
+    Q35_PIN();
+    tile += stride;
   }
 
-  // The waves' sums meet in LDS: row hr, dims (D / 16) (4 kg + e) + 4 g .. + 3
-  // of the lane's groups g.
-  __shared__ float o_s[NW][HP][D], ml_s[NW][HP][2];
+  // The waves' sums meet in LDS, each in its own ring: row hr, dims (D / 16) (4
+  // kg + e) + 4 g .. + 3 of the lane's groups g.
+  static_assert(HP * D * 4 <= F::RING, "a wave's sums fit its ring");
   l = kvq_col_sum(l);
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -692,7 +748,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
         for (int g = 1; g < GT; ++g) v[x] = gl == g ? o[4 * (ct * GT + g) + x][e] : v[x];
         v[x] += add;
       }
-      *reinterpret_cast<float4*>(&o_s[w][hr][NT * (4 * kg + e) + 4 * (ct * GT + gl)]) =
+      *reinterpret_cast<float4*>(ring + 4 * (hr * D + NT * (4 * kg + e) + 4 * (ct * GT + gl))) =
           make_float4(v[0], v[1], v[2], v[3]);
     }
   }
@@ -713,7 +769,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
 #pragma unroll
     for (int v = 0; v < NW; ++v) {
       const float f = __builtin_amdgcn_exp2f(ml_s[v][h][0] - ms);  // 0 for a wave without keys
-      const float4 t = *reinterpret_cast<const float4*>(&o_s[v][h][d]);
+      const float4 t = *reinterpret_cast<const float4*>(lds + v * F::RING + 4 * (h * D + d));
       sum.x = fmaf(t.x, f, sum.x); sum.y = fmaf(t.y, f, sum.y);
       sum.z = fmaf(t.z, f, sum.z); sum.w = fmaf(t.w, f, sum.w);
       ll = fmaf(ml_s[v][h][1], f, ll);
