@@ -340,12 +340,14 @@ struct KvqArgs {
   float scale;
   uint16_t* out;
   float* part;
-  int QH, KVH, L, C, blocks, splits, units;  // units = B * KVH * splits
+  int QH, KVH, L, C, blocks, splits, G, R;  // G = QH / KVH, R = G * L
 };
 
-// Keys that row r (head r % G of token r / G) of sequence b sees.
-Q35_DEV int kvq_limit(const KvqArgs& a, long long start, int r, int G) {
-  const long long n = start + r / G + 1;
+// Row r is head r % G of token r / G; a decoded token's rows need no division.
+Q35_DEV int kvq_token(const KvqArgs& a, int r) { return a.L == 1 ? 0 : (int)((unsigned)r / (unsigned)a.G); }
+// Keys that token i of a sequence that starts at `start` sees.
+Q35_DEV int kvq_limit(const KvqArgs& a, long long start, int i) {
+  const long long n = start + i + 1;
   return (int)(n < 0 ? 0 : n > a.C ? a.C : n);
 }
 Q35_DEV long long kvq_start(const KvqArgs& a, int b) {
@@ -411,12 +413,15 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   const int c16 = lane & 15, kg = lane >> 4, hr = c16 / GT, gl = c16 % GT;
   // Blocks of the same keys are 8 workgroups apart (one XCD, one L2) and next
   // in turn.
-  const int u = (int)(blockIdx.x / (8u * a.blocks)) * 8 + (int)(blockIdx.x % 8u);
-  const int blk = (int)(blockIdx.x / 8u) % a.blocks;
-  const int bh = u / a.splits, split = u % a.splits;
-  if (u >= a.units) return;  // the grid is rounded up to 8 units
-  const int b = bh / a.KVH, kvh = bh % a.KVH;
-  const int G = a.QH / a.KVH, R = G * a.L;
+  int split = blockIdx.x, blk = 0;
+  if (a.blocks > 1) {
+    const int x8 = split / 8;
+    blk = x8 % a.blocks;
+    split = x8 / a.blocks * 8 + split % 8;
+    if (split >= a.splits) return;
+  }
+  const int kvh = blockIdx.y, b = blockIdx.z, bh = b * a.KVH + kvh;
+  const int G = a.G, R = a.R;
 
   __shared__ alignas(1024) uint8_t lds[NW * F::RING + F::QB];
   __shared__ float ml_s[NW][HP][2];
@@ -431,9 +436,9 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   for (int z = 0; z < (F::QB + 1024 * NW - 1) / (1024 * NW); ++z) {
     const int at = 1024 * (w + NW * z);
     if (at < F::QB) {
-      const int r = min(row0 + (at + 16 * lane) / (2 * D), R - 1);
+      const int r = min(row0 + (at + 16 * lane) / (2 * D), R - 1), i = kvq_token(a, r);
       kvq_copy(__builtin_amdgcn_readfirstlane(lds_offset(q_raw + at)),
-               (const uint8_t*)(a.q + (((size_t)b * a.QH + kvh * G + r % G) * a.L + r / G) * D) +
+               (const uint8_t*)(a.q + (((size_t)b * a.QH + kvh * G + (r - i * G)) * a.L + i) * D) +
                    (at + 16 * lane) % (2 * D));
     }
   }
@@ -466,10 +471,9 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
 #pragma unroll
     for (int z = 0; z < F::NK; ++z) dma16(to + 1024 * (F::NK + z), vb, v_at[z]);
   };
-  const int r = min(row0 + hr, R - 1);
-  const int limit = kvq_limit(a, start, r, G);
-  const int least = kvq_limit(a, start, row0, G);
-  const int n_max = kvq_limit(a, start, min(row0 + HP, R) - 1, G);
+  const int limit = kvq_limit(a, start, kvq_token(a, min(row0 + hr, R - 1)));
+  const int least = kvq_limit(a, start, kvq_token(a, row0));
+  const int n_max = kvq_limit(a, start, kvq_token(a, min(row0 + HP, R) - 1));
   const int n_tiles = (n_max + 31) / 32;
   const int stride = a.splits * NW;
   int tile = split * NW + w;
@@ -570,19 +574,18 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   const q35_u32x4 ones = {offs, offs, offs, offs};
 
   auto step = [&](const Tile& t, int key0) {
-    float s[8];
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int ct = 0; ct < CT; ++ct) {
+      const float z = -F::OFF * qs[ct];
+      q35_f32x4 acc[2] = {{z, z, z, z}, {z, z, z, z}};
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const float z = -F::OFF * qs[ct];
-        q35_f32x4 acc = {z, z, z, z};
+      for (int x = 0; x < GT; ++x) {
+        const int g = ct * GT + x;
 #pragma unroll
-        for (int x = 0; x < GT; ++x) {
-          const int g = ct * GT + x;
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int tt = 0; tt < 2; ++tt) {
             q35_u32x4 kf;
             if constexpr (BITS == 4) {
               const uint32_t kw = t.k[tt][g][h];
@@ -591,23 +594,21 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
               const uint32_t k0 = t.k[tt][g][2 * h], k1 = t.k[tt][g][2 * h + 1];
               kf = q35_u32x4{kvq_pair8<0>(k0, k1), kvq_pair8<1>(k0, k1), kvq_pair8<2>(k0, k1), kvq_pair8<3>(k0, k1)};
             }
-            acc = mfma16(kf, qf[g][h], acc);
+            acc[tt] = mfma16(kf, qf[g][h], acc[tt]);
           }
-        }
-        const uint32_t(&pw)[4] = t.kp[tt][ct];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float st = bf_lo(pw[i]);
-          part[i] = fmaf(st, acc[i], fmaf(fmaf(F::HALF, st, bf_hi(pw[i])), qs[ct], part[i]));
-        }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = part[i];
-        if constexpr (GT > 1) x += dpp_f<Q35_DPP_QUAD_XOR1>(x);
-        if constexpr (GT > 2) x += dpp_f<Q35_DPP_QUAD_XOR2>(x);
-        s[4 * tt + i] = x * c2;
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t pw = t.kp[j >> 2][ct][j & 3];
+        const float st = bf_lo(pw);
+        s[j] = fmaf(st, acc[j >> 2][j & 3], fmaf(fmaf(F::HALF, st, bf_hi(pw)), qs[ct], s[j]));
       }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (GT > 1) s[j] += dpp_f<Q35_DPP_QUAD_XOR1>(s[j]);
+      if constexpr (GT > 2) s[j] += dpp_f<Q35_DPP_QUAD_XOR2>(s[j]);
+      s[j] *= c2;
     }
     float vs[CT][8], vm[CT][8];
 #pragma unroll
@@ -674,43 +675,31 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
       cnt[ct] = mfma16(ones, af[ct], cnt[ct]);
       cnt[ct] = mfma16(ones, al[ct], cnt[ct]);
     }
-    if constexpr (BITS == 4) {
+    // Four dims a turn (one group): the hi parts' products, then the lo parts'.
 #pragma unroll
-      for (int x = 0; x < VR; ++x) {
-        uint32_t lo[4], hi[4];
+    for (int g = 0; g < NT / 4; ++g) {
+      q35_u32x4 vf[4];
+      if constexpr (BITS == 4) {
+        const int x = g / 2;
+        const uint32_t sel = g & 1 ? 0x07060302u : 0x05040100u;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          lo[e] = __builtin_amdgcn_perm(t.v[2 * e + 1][x], t.v[2 * e][x], 0x05040100u);
-          hi[e] = __builtin_amdgcn_perm(t.v[2 * e + 1][x], t.v[2 * e][x], 0x07060302u);
+          const uint32_t h = __builtin_amdgcn_perm(t.v[2 * e + 1][x], t.v[2 * e][x], sel);
+          vf[0][e] = kvq_pair4<0>(h, cm); vf[1][e] = kvq_pair4<1>(h, cm);
+          vf[2][e] = kvq_pair4<2>(h, cm); vf[3][e] = kvq_pair4<3>(h, cm);
         }
-        auto pv = [&](auto tag, const uint32_t (&h)[4], int i) {
-          constexpr int N = decltype(tag)::value;
-          const q35_u32x4 vf = {kvq_pair4<N>(h[0], cm), kvq_pair4<N>(h[1], cm), kvq_pair4<N>(h[2], cm), kvq_pair4<N>(h[3], cm)};
-          o[i] = mfma16(vf, af[i / 4 / GT], o[i]);
-          o[i] = mfma16(vf, al[i / 4 / GT], o[i]);
-        };
-        pv(std::integral_constant<int, 0>{}, lo, 8 * x); pv(std::integral_constant<int, 1>{}, lo, 8 * x + 1);
-        pv(std::integral_constant<int, 2>{}, lo, 8 * x + 2); pv(std::integral_constant<int, 3>{}, lo, 8 * x + 3);
-        if constexpr (NT > 4) {
-          pv(std::integral_constant<int, 0>{}, hi, 8 * x + 4); pv(std::integral_constant<int, 1>{}, hi, 8 * x + 5);
-          pv(std::integral_constant<int, 2>{}, hi, 8 * x + 6); pv(std::integral_constant<int, 3>{}, hi, 8 * x + 7);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t v0 = t.v[2 * e][g], v1 = t.v[2 * e + 1][g];
+          vf[0][e] = kvq_pair8<0>(v0, v1); vf[1][e] = kvq_pair8<1>(v0, v1);
+          vf[2][e] = kvq_pair8<2>(v0, v1); vf[3][e] = kvq_pair8<3>(v0, v1);
         }
       }
-    } else {
 #pragma unroll
-      for (int x = 0; x < VR; ++x) {
-        auto pv = [&](auto tag) {
-          constexpr int N = decltype(tag)::value;
-          q35_u32x4 vf;
+      for (int i = 0; i < 4; ++i) o[4 * g + i] = mfma16(vf[i], af[g / GT], o[4 * g + i]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) vf[e] = kvq_pair8<N>(t.v[2 * e][x], t.v[2 * e + 1][x]);
-          const int i = 4 * x + N;
-          o[i] = mfma16(vf, af[i / 4 / GT], o[i]);
-          o[i] = mfma16(vf, al[i / 4 / GT], o[i]);
-        };
-        pv(std::integral_constant<int, 0>{}); pv(std::integral_constant<int, 1>{});
-        pv(std::integral_constant<int, 2>{}); pv(std::integral_constant<int, 3>{});
-      }
+      for (int i = 0; i < 4; ++i) o[4 * g + i] = mfma16(vf[i], al[g / GT], o[4 * g + i]);
     }
   };
   // Two tiles in flight: a tile is read into registers whole, then its place
@@ -781,58 +770,66 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
 
 // Merge of the splits that had keys: o = sum_s o_s 2^(m_s - M) / sum_s l_s
 // 2^(m_s - M), M = max m_s. One workgroup a query row and 64 dims, 16 threads of
-// 4 dims by 16 parts of the splits, so a thread reads at most 16 records.
+// 4 dims by 16 parts of the splits, so a thread reads PER = splits / 16 records
+// of at most 256.
 constexpr int kKvqSplits = 256;
-template <int D, int HP>
+template <int D, int HP, int PER>
 __global__ __launch_bounds__(256) void kvq_few_merge(const KvqArgs a) {
   constexpr int NW = 4, REC = HP * (D + 2);
-  const int t = threadIdx.x, d = 64 * (int)blockIdx.y + 4 * (t & 15), part = t >> 4;
-  const int G = a.QH / a.KVH, R = G * a.L;
-  const int bh = blockIdx.x / (unsigned)R, r = blockIdx.x % (unsigned)R;
-  const int b = bh / a.KVH, kvh = bh % a.KVH, blk = r / HP, h = r % HP;
-  const long long start = kvq_start(a, b);
-  const int n_max = kvq_limit(a, start, min(blk * HP + HP, R) - 1, G);
-  const int n = min(a.splits, ((n_max + 31) / 32 + NW - 1) / NW);
+  const int t = threadIdx.x, part = t >> 4;
+  const int r = blockIdx.x / (D / 64), d = 64 * (int)(blockIdx.x % (D / 64)) + 4 * (t & 15);
+  const int kvh = blockIdx.y, b = blockIdx.z, bh = b * a.KVH + kvh, blk = r / HP, h = r % HP;
+  // Requested together: a part's records, the thread's split's (m, l) and the
+  // length that says which of them were written.
   const float* rec = a.part + (size_t)(bh * a.blocks + blk) * a.splits * REC;
+  const long long start = kvq_start(a, b);
+  const float2 raw = *reinterpret_cast<const float2*>(rec + (size_t)min(t, a.splits - 1) * REC + HP * D + 2 * h);
+  float4 x[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    x[j] = *reinterpret_cast<const float4*>(rec + (size_t)min(part + 16 * j, a.splits - 1) * REC + h * D + d);
+  const int i = kvq_token(a, r), head = kvh * a.G + (r - i * a.G);
+  const uint2 gate = a.gate ? *reinterpret_cast<const uint2*>(a.gate + b * a.gate_stride + (2 * head + 1) * D + d)
+                            : make_uint2(0, 0);
+  const int n_max = kvq_limit(a, start, kvq_token(a, min(blk * HP + HP, a.R) - 1));
+  const int n = min(a.splits, ((n_max + 31) / 32 + NW - 1) / NW);
   __shared__ float f_s[kKvqSplits], red_s[2][4];
   __shared__ float4 sum_s[16][16];
-  float2 ml = make_float2(-INFINITY, 0.f);
-  if (t < n) ml = *reinterpret_cast<const float2*>(rec + (size_t)t * REC + HP * D + 2 * h);
-  const float mw = wave_max(ml.x);
+  const float m = t < n ? raw.x : -INFINITY, l = t < n ? raw.y : 0.f;
+  const float mw = wave_max(m);
   if ((t & 63) == 0) red_s[0][t >> 6] = mw;
   __syncthreads();
   const float mm = fmaxf(fmaxf(red_s[0][0], red_s[0][1]), fmaxf(red_s[0][2], red_s[0][3]));
-  const float f = __builtin_amdgcn_exp2f(ml.x - (mm == -INFINITY ? 0.f : mm));
+  const float f = __builtin_amdgcn_exp2f(m - (mm == -INFINITY ? 0.f : mm));
   f_s[t] = f;
-  const float lw = wave_sum(ml.y * f);
+  const float lw = wave_sum(l * f);
   if ((t & 63) == 0) red_s[1][t >> 6] = lw;
   __syncthreads();
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = part; s < n; s += 16) {
-    const float4 x = *reinterpret_cast<const float4*>(rec + (size_t)s * REC + h * D + d);
-    const float fs = f_s[s];
-    sum.x = fmaf(x.x, fs, sum.x); sum.y = fmaf(x.y, fs, sum.y);
-    sum.z = fmaf(x.z, fs, sum.z); sum.w = fmaf(x.w, fs, sum.w);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (part + 16 * j < n) {  // not a weight of 0: what was not written may be anything
+      const float fs = f_s[part + 16 * j];
+      sum.x = fmaf(x[j].x, fs, sum.x); sum.y = fmaf(x[j].y, fs, sum.y);
+      sum.z = fmaf(x[j].z, fs, sum.z); sum.w = fmaf(x[j].w, fs, sum.w);
+    }
   }
   sum_s[part][t & 15] = sum;
   __syncthreads();
   if (part) return;
 #pragma unroll
   for (int v = 1; v < 16; ++v) {
-    const float4 x = sum_s[v][t];
-    sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+    const float4 y = sum_s[v][t];
+    sum.x += y.x; sum.y += y.y; sum.z += y.z; sum.w += y.w;
   }
   // a row without keys is zero
-  const float inv = kvq_limit(a, start, r, G) ? 1.0f / ((red_s[1][0] + red_s[1][1]) + (red_s[1][2] + red_s[1][3])) : 0.f;
-  const int head = kvh * G + r % G;
+  const float inv = kvq_limit(a, start, i) ? 1.0f / ((red_s[1][0] + red_s[1][1]) + (red_s[1][2] + red_s[1][3])) : 0.f;
   float v[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
   if (a.gate) {
-    const uint2 x = *reinterpret_cast<const uint2*>(a.gate + b * a.gate_stride + (2 * head + 1) * D + d);
-    v[0] *= sigmoid_f(bf_lo(x.x)); v[1] *= sigmoid_f(bf_hi(x.x));
-    v[2] *= sigmoid_f(bf_lo(x.y)); v[3] *= sigmoid_f(bf_hi(x.y));
+    v[0] *= sigmoid_f(bf_lo(gate.x)); v[1] *= sigmoid_f(bf_hi(gate.x));
+    v[2] *= sigmoid_f(bf_lo(gate.y)); v[3] *= sigmoid_f(bf_hi(gate.y));
   }
-  *reinterpret_cast<uint2*>(a.out + (((size_t)b * a.L + r / G) * a.QH + head) * D + d) =
+  *reinterpret_cast<uint2*>(a.out + (((size_t)b * a.L + i) * a.QH + head) * D + d) =
       make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
 }
 
@@ -940,19 +937,21 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
   if (rows <= kKvqFewRows) {
     const int hp = kvq_block_rows(D, rows), blocks = (int)((rows + hp - 1) / hp);
     const int splits = kvq_splits(B, KVH, blocks, capacity);
-    const long long units = (long long)B * KVH * splits;
-    Q35_CHECK_ARG(workspace && q35_aligned16(workspace) &&
-                  workspace_floats >= units * blocks * hp * (D + 2) && (units + 7) * blocks < (1ll << 31));
+    Q35_CHECK_ARG(B < 65536 && KVH < 65536 && workspace && q35_aligned16(workspace) &&
+                  workspace_floats >= (long long)B * KVH * splits * blocks * hp * (D + 2));
     const KvqArgs a{(const uint16_t*)q, (const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,
                     (const uint32_t*)vp, (const long long*)len_dev, n_len, offset, (const uint16_t*)gate, gate_stride,
-                    scale, (uint16_t*)out, (float*)workspace, QH, KVH, L, capacity, blocks, splits, (int)units};
-    const unsigned grid = (unsigned)((units + 7) / 8 * 8 * blocks);
-    const dim3 mgrid((unsigned)(B * KVH * rows), (unsigned)(D / 64));
-#define Q35_FEW(DD, HP)                                             \
-  do {                                                              \
-    if (bits == 4) kvq_few<DD, 4, HP><<<grid, 256, 0, stream>>>(a); \
-    else kvq_few<DD, 8, HP><<<grid, 256, 0, stream>>>(a);           \
-    kvq_few_merge<DD, HP><<<mgrid, 256, 0, stream>>>(a);            \
+                    scale, (uint16_t*)out, (float*)workspace, QH, KVH, L, capacity, blocks, splits, QH / KVH,
+                    (int)rows};
+    const dim3 grid((unsigned)(blocks == 1 ? splits : (splits + 7) / 8 * 8 * blocks), (unsigned)KVH, (unsigned)B);
+    const dim3 mgrid((unsigned)(rows * (D / 64)), (unsigned)KVH, (unsigned)B);
+#define Q35_FEW(DD, HP)                                                            \
+  do {                                                                             \
+    if (bits == 4) kvq_few<DD, 4, HP><<<grid, 256, 0, stream>>>(a);                \
+    else kvq_few<DD, 8, HP><<<grid, 256, 0, stream>>>(a);                          \
+    if (splits <= 16) kvq_few_merge<DD, HP, 1><<<mgrid, 256, 0, stream>>>(a);      \
+    else if (splits <= 64) kvq_few_merge<DD, HP, 4><<<mgrid, 256, 0, stream>>>(a); \
+    else kvq_few_merge<DD, HP, 16><<<mgrid, 256, 0, stream>>>(a);                  \
   } while (0)
     if (D == 64) Q35_FEW(64, 16);
     else if (D == 128 && hp == 8) Q35_FEW(128, 8);
