@@ -19,13 +19,9 @@
 // Layouts: codes [B, KVH, C, D * bits / 8] bytes, dims in order, in 4 bits the
 // even dim in a byte's low half; params [B, KVH, D / 64, C] pairs of bf16
 // (step in the low half of a 32-bit word, low in the high half).
-#include <type_traits>
-
-#include "q35_tile.hpp"
+#include "kvq.hpp"
 
 namespace {
-
-Q35_DEV uint32_t kvq_code(uint32_t w, int i, int bits) { return bits == 4 ? (w >> (4 * i)) & 15u : (w >> (8 * i)) & 255u; }
 
 // Whether a code's place between its neighbours has to be looked at exactly:
 // t = (x - low) / step less the code, as computed with a reciprocal (relative
@@ -170,116 +166,6 @@ __global__ __launch_bounds__(256) void kvq_write(const KvqSrc ks, const KvqSrc v
   }
 }
 
-// ---------------------------------------------------------------- read back
-// The same 16 lanes a row: bf16(fma(code, step, low)), one rounding.
-template <int E, int BITS>
-__global__ __launch_bounds__(256) void kvq_read(const uint8_t* __restrict__ kq, const uint8_t* __restrict__ vq,
-                                                const uint32_t* __restrict__ kp, const uint32_t* __restrict__ vp,
-                                                uint16_t* __restrict__ k, uint16_t* __restrict__ v, int start,
-                                                int L, int C, unsigned rows) {
-  constexpr int NG = E / 4, RB = 2 * E * BITS;
-  const unsigned row = blockIdx.x * 16u + (threadIdx.x >> 4);
-  if (row >= rows) return;
-  const int c = threadIdx.x & 15;
-  const unsigned bh = row / (unsigned)L, pos = start + row % (unsigned)L;
-  const bool values = blockIdx.y != 0;
-  const uint8_t* src = (values ? vq : kq) + ((size_t)bh * C + pos) * RB + c * (E * BITS / 8);
-  const uint32_t* ps = (values ? vp : kp) + (size_t)bh * NG * C + pos;
-  uint32_t w[(E * BITS + 31) / 32];
-  if constexpr (E * BITS == 16) w[0] = *reinterpret_cast<const uint16_t*>(src);
-  else if constexpr (E * BITS == 32) w[0] = *reinterpret_cast<const uint32_t*>(src);
-  else if constexpr (E * BITS == 64) {
-    const uint2 a = *reinterpret_cast<const uint2*>(src);
-    w[0] = a.x; w[1] = a.y;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(src);
-    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-  }
-  uint32_t p[NG];
-#pragma unroll
-  for (int g = 0; g < NG; ++g) p[g] = ps[(size_t)(values ? g : c * E / 64) * C];
-  uint32_t o[E / 2];
-#pragma unroll
-  for (int e = 0; e < E; e += 2) {
-    const uint32_t pw = p[e / 4];
-    const float st = bf_lo(pw), lw = bf_hi(pw);
-    const float a = fmaf((float)kvq_code(w[e * BITS / 32], e % (32 / BITS), BITS), st, lw);
-    const float d = fmaf((float)kvq_code(w[e * BITS / 32], e % (32 / BITS) + 1, BITS), st, lw);
-    o[e / 2] = pack_bf2(a, d);
-  }
-  uint16_t* dst = (values ? v : k) + (size_t)row * (16 * E) + E * c;
-  if constexpr (E == 4) {
-    *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < E / 8; ++j)
-      *reinterpret_cast<uint4*>(dst + 8 * j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-  }
-}
-
-// ---------------------------------------------------------------- attention
-// One wave a (batch, head, query row): lane l holds the V of its P = D / 64
-// dims P l .., every key's score is reduced over the wave, online softmax in
-// fp32. Row i of a sequence sees keys 0 .. start + i.
-template <int P, int BITS>
-__global__ __launch_bounds__(256) void kvq_attend_rows(
-    const uint16_t* __restrict__ q, const uint8_t* __restrict__ kq, const uint8_t* __restrict__ vq,
-    const uint32_t* __restrict__ kp, const uint32_t* __restrict__ vp, const long long* len_dev, int n_len,
-    long long offset, const uint16_t* __restrict__ gate, long long gate_stride, float scale,
-    uint16_t* __restrict__ out, int QH, int KVH, int L, int C, long long rows) {
-  constexpr int D = 64 * P, NG = P, RB = D * BITS / 8;
-  const int lane = threadIdx.x & 63;
-  const long long wv = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (wv >= rows) return;
-  const int i = L - 1 - (int)(wv % L);
-  const int h = (int)(wv / L % QH);
-  const int b = (int)(wv / L / QH);
-  const size_t bh = (size_t)b * KVH + h / (QH / KVH);
-  const long long at = (len_dev ? len_dev[n_len > 1 ? b : 0] : 0) + offset + i + 1;
-  const int n = (int)(at < 0 ? 0 : at > C ? C : at);
-  const uint16_t* qr = q + (((size_t)b * QH + h) * L + i) * D + P * lane;
-  float qf[P], acc[P];
-  int vg[P];
-#pragma unroll
-  for (int e = 0; e < P; ++e) {
-    qf[e] = bf2f(qr[e]);
-    acc[e] = 0.f;
-    vg[e] = (P * lane + e) % (4 * P) / 4;
-  }
-  const int kg = P * lane / 64;
-  const uint8_t* K = kq + bh * C * RB;
-  const uint8_t* V = vq + bh * C * RB;
-  const uint32_t* KP = kp + (bh * NG + kg) * C;
-  const uint32_t* VP = vp + bh * NG * C;
-  float m = -INFINITY, l = 0.f;
-  auto code = [&](const uint8_t* base, int t, int d) {
-    return BITS == 4 ? (float)((base[(size_t)t * RB + d / 2] >> (4 * (d & 1))) & 15) : (float)base[(size_t)t * RB + d];
-  };
-  for (int t = 0; t < n; ++t) {
-    const uint32_t kw = KP[t];
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < P; ++e) s = fmaf(qf[e], fmaf(code(K, t, P * lane + e), bf_lo(kw), bf_hi(kw)), s);
-    s = wave_sum(s) * scale;
-    const float mn = fmaxf(m, s);
-    const float corr = expf(m - mn), p = expf(s - mn);
-    l = l * corr + p;
-#pragma unroll
-    for (int e = 0; e < P; ++e) {
-      const uint32_t vw = VP[(size_t)vg[e] * C + t];
-      acc[e] = fmaf(p, fmaf(code(V, t, P * lane + e), bf_lo(vw), bf_hi(vw)), acc[e] * corr);
-    }
-    m = mn;
-  }
-#pragma unroll
-  for (int e = 0; e < P; ++e) {
-    const int d = P * lane + e;
-    float o = n ? acc[e] / l : 0.f;  // a row without keys is zero
-    if (gate) o *= sigmoid_f(bf2f(gate[b * gate_stride + (2 * h + 1) * D + d]));
-    out[(((size_t)b * L + i) * QH + h) * D + d] = (uint16_t)f2bf(o);
-  }
-}
-
 // ------------------------------------------------- attention of a few rows
 // The query rows of one KV head, G = QH / KVH heads x L tokens, in blocks of HP
 // rows; a workgroup takes one block and every S-th piece of NW x 32 keys, a
@@ -327,32 +213,6 @@ struct KvqFew {
     uint32_t k[2][NG][KW], v[8][VR], kp[2][CT][4], vp[2][CT][4];
   };
 };
-
-struct KvqArgs {
-  const uint16_t* q;
-  const uint8_t *kq, *vq;
-  const uint32_t *kp, *vp;
-  const long long* len;
-  int n_len;
-  long long offset;
-  const uint16_t* gate;
-  long long gate_stride;
-  float scale;
-  uint16_t* out;
-  float* part;
-  int QH, KVH, L, C, blocks, splits, G, R;  // G = QH / KVH, R = G * L
-};
-
-// Row r is head r % G of token r / G; a decoded token's rows need no division.
-Q35_DEV int kvq_token(const KvqArgs& a, int r) { return a.L == 1 ? 0 : (int)((unsigned)r / (unsigned)a.G); }
-// Keys that token i of a sequence that starts at `start` sees.
-Q35_DEV int kvq_limit(const KvqArgs& a, long long start, int i) {
-  const long long n = start + i + 1;
-  return (int)(n < 0 ? 0 : n > a.C ? a.C : n);
-}
-Q35_DEV long long kvq_start(const KvqArgs& a, int b) {
-  return (a.len ? a.len[a.n_len > 1 ? b : 0] : 0) + a.offset;
-}
 
 // One wave instruction of a copy: lane i's 16 bytes at p to LDS bytes [lds + 16
 // i, +16).
@@ -907,8 +767,8 @@ int q35_kv_dequantize(const void* kq, const void* vq, const void* kp, const void
   const dim3 grid((unsigned)((rows + 15) / 16), 2);
 #define Q35_CALL(E, BITS)                                                                                          \
   kvq_read<E, BITS><<<grid, 256, 0, stream>>>((const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,          \
-                                              (const uint32_t*)vp, (uint16_t*)k, (uint16_t*)v, start, L, capacity,  \
-                                              (unsigned)rows)
+                                              (const uint32_t*)vp, (uint16_t*)k, (uint16_t*)v, start, L, L,         \
+                                              capacity, (unsigned)rows, nullptr, 0, 0, KVH)
   Q35_KVQ_BY_D(Q35_CALL);
 #undef Q35_CALL
   return q35_last_error();
@@ -917,7 +777,8 @@ int q35_kv_dequantize(const void* kq, const void* vq, const void* kp, const void
 long long q35_gqa_attention_kvq_workspace(int B, int QH, int KVH, int L, int D, int bits, int capacity) {
   if (!kvq_shape_ok(B, KVH, L, D, bits, capacity) || QH <= 0 || QH % KVH) return -1;
   const long long rows = (long long)(QH / KVH) * L;
-  if ((long long)B * L == 0 || rows > kKvqFewRows) return 0;
+  if ((long long)B * L == 0) return 0;
+  if (rows > kKvqFewRows) return kvq_prompt_workspace(B, QH, KVH, L, D, capacity);
   const int hp = kvq_block_rows(D, rows), blocks = (int)((rows + hp - 1) / hp);
   return (long long)B * KVH * blocks * kvq_splits(B, KVH, blocks, capacity) * hp * (D + 2);
 }
@@ -962,16 +823,10 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
 #undef Q35_FEW
     return q35_last_error();
   }
-  const long long waves = (long long)B * QH * L;
-  const unsigned grid = (unsigned)((waves + 3) / 4);
-#define Q35_CALL(E, BITS)                                                                                           \
-  kvq_attend_rows<E / 4, BITS><<<grid, 256, 0, stream>>>(                                                           \
-      (const uint16_t*)q, (const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp, (const uint32_t*)vp,          \
-      (const long long*)len_dev, n_len, offset, (const uint16_t*)gate, gate_stride, scale, (uint16_t*)out, QH, KVH,  \
-      L, capacity, waves)
-  Q35_KVQ_BY_D(Q35_CALL);
-#undef Q35_CALL
-  return q35_last_error();
+  Q35_CHECK_ARG(workspace && q35_aligned16(workspace) &&
+                workspace_floats >= kvq_prompt_workspace(B, QH, KVH, L, D, capacity));
+  return kvq_prompt(q, kq, vq, kp, vp, (const long long*)len_dev, n_len, offset, scale, out, (float*)workspace, B, QH,
+                    KVH, L, D, bits, capacity, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,93 @@
+// What the kernels of the K/V cache in 4 or 8 bits share: its form is described in
+// kvq.hip.
+#pragma once
+#include "q35_tile.hpp"
+
+namespace {
+
+Q35_DEV uint32_t kvq_code(uint32_t w, int i, int bits) { return bits == 4 ? (w >> (4 * i)) & 15u : (w >> (8 * i)) & 255u; }
+
+struct KvqArgs {
+  const uint16_t* q;
+  const uint8_t *kq, *vq;
+  const uint32_t *kp, *vp;
+  const long long* len;
+  int n_len;
+  long long offset;
+  const uint16_t* gate;
+  long long gate_stride;
+  float scale;
+  uint16_t* out;
+  float* part;
+  int QH, KVH, L, C, blocks, splits, G, R;  // G = QH / KVH, R = G * L
+};
+
+// Row r is head r % G of token r / G; a decoded token's rows need no division.
+Q35_DEV int kvq_token(const KvqArgs& a, int r) { return a.L == 1 ? 0 : (int)((unsigned)r / (unsigned)a.G); }
+// Keys that token i of a sequence that starts at `start` sees.
+Q35_DEV int kvq_limit(const KvqArgs& a, long long start, int i) {
+  const long long n = start + i + 1;
+  return (int)(n < 0 ? 0 : n > a.C ? a.C : n);
+}
+Q35_DEV long long kvq_start(const KvqArgs& a, int b) {
+  return (a.len ? a.len[a.n_len > 1 ? b : 0] : 0) + a.offset;
+}
+
+// ---------------------------------------------------------------- read back
+// The same 16 lanes a row: bf16(fma(code, step, low)), one rounding. Rows start ..
+// start + L - 1 of every head go to rows of `stride` a head; with a length on
+// the device only the rows that a sequence's last token sees.
+template <int E, int BITS>
+__global__ __launch_bounds__(256) void kvq_read(const uint8_t* __restrict__ kq, const uint8_t* __restrict__ vq,
+                                                const uint32_t* __restrict__ kp, const uint32_t* __restrict__ vp,
+                                                uint16_t* __restrict__ k, uint16_t* __restrict__ v, int start,
+                                                int L, int stride, int C, unsigned rows, const long long* len,
+                                                int n_len, long long last, int KVH) {
+  constexpr int NG = E / 4, RB = 2 * E * BITS;
+  const unsigned row = blockIdx.x * 16u + (threadIdx.x >> 4);
+  if (row >= rows) return;
+  const int c = threadIdx.x & 15;
+  const unsigned bh = row / (unsigned)L, at = row % (unsigned)L, pos = start + at;
+  if (len && (long long)pos > len[n_len > 1 ? bh / (unsigned)KVH : 0] + last) return;
+  const bool values = blockIdx.y != 0;
+  const uint8_t* src = (values ? vq : kq) + ((size_t)bh * C + pos) * RB + c * (E * BITS / 8);
+  const uint32_t* ps = (values ? vp : kp) + (size_t)bh * NG * C + pos;
+  uint32_t w[(E * BITS + 31) / 32];
+  if constexpr (E * BITS == 16) w[0] = *reinterpret_cast<const uint16_t*>(src);
+  else if constexpr (E * BITS == 32) w[0] = *reinterpret_cast<const uint32_t*>(src);
+  else if constexpr (E * BITS == 64) {
+    const uint2 a = *reinterpret_cast<const uint2*>(src);
+    w[0] = a.x; w[1] = a.y;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(src);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+  }
+  uint32_t p[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) p[g] = ps[(size_t)(values ? g : c * E / 64) * C];
+  uint32_t o[E / 2];
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    const uint32_t pw = p[e / 4];
+    const float st = bf_lo(pw), lw = bf_hi(pw);
+    const float a = fmaf((float)kvq_code(w[e * BITS / 32], e % (32 / BITS), BITS), st, lw);
+    const float d = fmaf((float)kvq_code(w[e * BITS / 32], e % (32 / BITS) + 1, BITS), st, lw);
+    o[e / 2] = pack_bf2(a, d);
+  }
+  uint16_t* dst = (values ? v : k) + ((size_t)bh * stride + at) * (16 * E) + E * c;
+  if constexpr (E == 4) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < E / 8; ++j)
+      *reinterpret_cast<uint4*>(dst + 8 * j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+  }
+}
+
+}  // namespace
+
+// Attention of many query rows (kvq_prompt.hip): workspace floats and launch.
+long long kvq_prompt_workspace(int B, int QH, int KVH, int L, int D, int C);
+int kvq_prompt(const void* q, const void* kq, const void* vq, const void* kp, const void* vp, const long long* len,
+               int n_len, long long offset, float scale, void* out, float* workspace, int B, int QH, int KVH, int L,
+               int D, int bits, int C, hipStream_t stream);

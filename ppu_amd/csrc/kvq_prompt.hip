@@ -1,0 +1,525 @@
+// Causal GQA attention of many query rows over the K/V cache in 4 or 8 bits: the
+// cache's values as bf16 in a workspace, one pass over them (kvq_read), and
+// flash attention on the matrix cores over those.
+//
+// A row tile of 128 rows reads every key once, so a prompt of n rows would
+// unpack a cache n / 128 times inside the attention; unpacked once, its blocks
+// go from memory straight into LDS. The values are rounded to bf16 as a bf16
+// cache holds them, a 2^-8 error at most against a 4-bit step of a fifteenth of
+// the group's range.
+#include "kvq.hpp"
+
+namespace {
+
+Q35_DEV uint2 lds_read_tr16(const void* p) {
+  typedef short q35_i16x4 __attribute__((ext_vector_type(4)));
+  const q35_i16x4 v =
+      __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) q35_i16x4*)(p));
+  return __builtin_bit_cast(uint2, v);
+}
+
+constexpr int kFaKeys = 64;       // keys per block
+constexpr int kFaWaves = 4;
+constexpr int kFaRows = 32 * kFaWaves;  // query rows per tile
+constexpr int kFaMaxSplits = 64;
+
+template <int D>
+struct FaShape {
+  static constexpr int ROW = 2 * D;                  // bytes of a K or V row
+  static constexpr int BLOCK = kFaKeys * ROW;        // of a block
+  static constexpr int CPR = ROW / 16;               // 16-byte chunks of a row
+  static constexpr int NC = BLOCK / 1024 / kFaWaves; // a wave's copies of a block
+  static constexpr int KS = D / 16, ND = D / 32;     // k steps of S, dim tiles of O
+  static constexpr int REC = 32 * (D + 2);           // floats of a wave's split record
+  static constexpr int WAVES = D > 64 ? 1 : 2;     // waves a SIMD
+};
+
+// 16-byte chunk c of a staged row r sits at slot c ^ fa_swz(r): the 16 rows of a
+// K fragment read and the 4 rows x 4 chunks of a transposed V read each fall on
+// 16 distinct bank groups.
+template <int D>
+Q35_DEV uint32_t fa_swz(uint32_t r) {
+  if (D == 64) {
+    const uint32_t x = r >> 1 & 7;
+    return ((x & 1) << 2) | (x >> 1);
+  }
+  return ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
+struct FaArgs {
+  const uint16_t *q, *K, *V;  // K, V [B * KVH, stride, D]
+  const long long* len;
+  int n_len;
+  long long offset;
+  float scale;
+  uint16_t* out;
+  float* part;
+  int QH, KVH, L, C, stride, G, R, tiles, splits, bhs;
+};
+Q35_DEV long long fa_start(const FaArgs& a, int b) { return (a.len ? a.len[a.n_len > 1 ? b : 0] : 0) + a.offset; }
+// Keys that row r sees.
+Q35_DEV int fa_limit(const FaArgs& a, long long start, int r) {
+  const long long n = start + (int)((unsigned)r / (unsigned)a.G) + 1;
+  return (int)(n < 0 ? 0 : n > a.C ? a.C : n);
+}
+// Key blocks per range of a tile with nblk of them: over at most `splits`
+// ranges, of at least two blocks.
+Q35_DEV int fa_range(const FaArgs& a, int nblk) { return max((nblk + a.splits - 1) / a.splits, min(nblk, 2)); }
+
+template <bool V> struct FaTag { static constexpr bool value = V; };
+
+// ------------------------------------------------- attention of many rows
+// Products are transposed: a wave owns 32 query rows (row = token x head of one
+// KV head, so any head grouping fills its tiles) as the COLUMNS of every
+// v_mfma_f32_32x32x16_bf16,
+//   S^T = K Q^T  (A = 32 keys x 16 dims from LDS, B = Q^T held in registers),
+//   O^T += V^T P^T  (A = 32 dims x 16 keys from LDS, B = P^T),
+// so a lane holds one query row: the softmax needs no cross-lane step but one
+// exchange between lanes l and l ^ 32 per block, and the C layout of S^T is,
+// with the 16 keys of a k step taken in the order {0-3, 8-11 | 4-7, 12-15},
+// already the B operand of O^T: P, rounded to bf16, never leaves the registers.
+// V rows reach the A operand through the transpose read ds_read_b64_tr_b16:
+// within a 16-lane group, lane 4 e + q points at row e, column 4 q and lane i
+// receives the 4 rows of column i.
+//
+// The 4 waves of a workgroup are 4 tiles of 32 rows that share the K and V
+// blocks in LDS (two buffers each, rows copied straight into LDS a whole block
+// ahead, one barrier per block). Vector work is interleaved by hand: the MFMAs
+// of S for block j + 1 carry the copies of the following blocks and half of the
+// exponentials of block j, the MFMAs of O the other half, the packing of P and
+// the scale and row maximum of block j + 1.
+//
+// The running maximum m (in units of log2) moves only when a row's block maximum
+// passes it by 8: P stays below 2^8 and O is rescaled a few times per row.
+//
+// Keys past a tile's last one are clamped to it on load and, like every key
+// past a row's own end, masked to -inf in S. In blocks where some row's end
+// lies, V's infinities and NaN are taken out and their dims set to NaN at the
+// end for the rows that see them: a weight of zero would not hide them.
+template <int D>
+__global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(const FaArgs a) {
+  using F = FaShape<D>;
+  constexpr int KS = F::KS, ND = F::ND, NC = F::NC, ROW = F::ROW, BLOCK = F::BLOCK;
+  // K buffers at 0 and BLOCK, V buffers at 2 and 3 BLOCK
+  __shared__ alignas(1024) uint8_t lds[4 * BLOCK];
+  __shared__ int bad_s[D];  // first key of a masked block with a dim's V not finite
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int l32 = lane & 31, kh = lane >> 5;
+  // The last split of every tile, late tiles first, down to split 0, which is
+  // the rest: the longest ranges start first.
+  const int bh = (int)(blockIdx.x % (unsigned)a.bhs), at = (int)(blockIdx.x / (unsigned)a.bhs);
+  const int tile = a.tiles - 1 - at % a.tiles, split = a.splits - 1 - at / a.tiles;
+  const int b = bh / a.KVH, kvh = bh % a.KVH;
+  const int r0 = tile * kFaRows, rw = r0 + 32 * w;
+  const long long start = fa_start(a, b);
+  const int n_keys = fa_limit(a, start, min(r0 + kFaRows, a.R) - 1);
+  const int nblk = (n_keys + kFaKeys - 1) / kFaKeys;
+  const int sb = fa_range(a, nblk), nsplit = nblk ? (nblk + sb - 1) / sb : 1;
+  if (split >= nsplit) return;  // whole workgroup: no barrier is skipped
+  const int row = min(rw + l32, a.R - 1);
+  const int tok = (int)((unsigned)row / (unsigned)a.G), head = kvh * a.G + (row - tok * a.G);
+  uint16_t* orow = a.out + (((size_t)b * a.L + tok) * a.QH + head) * D;
+  if (nblk == 0) {  // no row of the tile sees a key
+    if (rw + l32 < a.R)
+      for (int d = 8 * kh; d < D; d += 16) *reinterpret_cast<uint4*>(orow + d) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int b1 = nblk - (nsplit - 1 - split) * sb, b0 = split ? b1 - sb : 0;
+  const uint8_t* Kh = (const uint8_t*)(a.K + (size_t)bh * a.stride * D);
+  const uint8_t* Vh = (const uint8_t*)(a.V + (size_t)bh * a.stride * D);
+
+  // ---- copies: wave w takes 1 KiB pieces w + 4 i of each block
+  const uint32_t cr = (1024u / ROW) * w + lane / F::CPR, cstep = 4u * (1024u / ROW);  // row of copy i: cr + cstep i
+  const uint32_t cc[2] = {16u * ((uint32_t)(lane % F::CPR) ^ fa_swz<D>(cr)),
+                          16u * ((uint32_t)(lane % F::CPR) ^ fa_swz<D>(cr + cstep))};
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_offset(lds) + 1024u * (uint32_t)w);
+  auto copy = [&](const uint8_t* base, uint32_t to, int blk, int i) {
+    const uint32_t r = min(cr + cstep * i, (uint32_t)(n_keys - 1 - blk * kFaKeys));
+    dma16(lds0 + to + 4096u * i, base + (size_t)blk * BLOCK, r * ROW + cc[i & 1]);
+  };
+
+  // ---- fragment addresses; the buffer is added by ^ BLOCK
+  // K: row l32 of a 32-key half (the second half BLOCK / 2 on), chunk 2 s + kh
+  uint32_t ka[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) ka[s] = (uint32_t)l32 * ROW + 16u * ((2u * s + kh) ^ fa_swz<D>(l32));
+  // V: rows 4 kh + e and 4 kh + 8 + e of a 16-key step, dims 32 d + 16 ((lane /
+  // 16) % 2) + 4 (lane % 4)
+  uint32_t va[2][ND];
+  {
+    const uint32_t e = (lane & 15) >> 2, cl = 2u * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t r = 4u * kh + 8u * u + e;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        va[u][d] = 2u * BLOCK + r * ROW + 16u * ((4u * d + cl) ^ fa_swz<D>(r)) + 8u * (lane & 1);
+    }
+  }
+
+  // ---- Q: column l32 of the B operand, dims 16 s + 8 kh ..
+  q35_u32x4 qf[KS];
+  {
+    const uint16_t* qp = a.q + (((size_t)b * a.QH + head) * a.L + tok) * D + 8 * kh;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const q35_u32x4*>(qp + 16 * s);
+  }
+  const int limit = fa_limit(a, start, row);
+  const int least = fa_limit(a, start, min(rw, a.R - 1));     // of the wave's rows
+  const int least_wg = fa_limit(a, start, r0);                // of the workgroup's
+  const float c2 = a.scale * 1.4426950408889634f;
+  bool bad = false;
+
+  q35_f32x16 o[ND], sc[2], sn[2];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m = -INFINITY, l = 0.f, mx = -INFINITY;
+
+  // ---- prologue: K and V of the first block, K of the second; S of the first
+#pragma unroll
+  for (int i = 0; i < NC; ++i) copy(Kh, 0, b0, i);
+#pragma unroll
+  for (int i = 0; i < NC; ++i) copy(Vh, 2u * BLOCK, b0, i);
+#pragma unroll
+  for (int i = 0; i < NC; ++i) copy(Kh, BLOCK, min(b0 + 1, b1 - 1), i);
+  wait_vm<2 * NC>();
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sn[t][r] = 0.f;
+#pragma unroll
+  for (int x = 0; x < 2 * KS; ++x)
+    sn[x & 1] = mfma32(*reinterpret_cast<const q35_u32x4*>(lds + ka[x >> 1] + (BLOCK / 2) * (x & 1)), qf[x >> 1], sn[x & 1]);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      sc[t][r] = sn[t][r] * c2;
+      mx = fmaxf(mx, sc[t][r]);
+    }
+#pragma unroll
+  for (int s = 0; s < KS; ++s) ka[s] ^= (uint32_t)BLOCK;
+  wait_vm<0>();
+  __syncthreads();
+
+  // ---- one block: sc holds its scaled scores, mx their maximum over the
+  // lane's keys; ka points at K of the next block, va at V of this one
+  auto block = [&](int blk, auto next_tag) {
+    constexpr bool NEXT = decltype(next_tag)::value;
+    const uint32_t kbuf = (blk - b0) & 1 ? BLOCK : 0;  // free: this block's K, the last one's V
+    const uint32_t vbuf = 2u * BLOCK + (BLOCK - kbuf);
+    if (blk * kFaKeys + kFaKeys > least_wg) {  // uniform over the workgroup
+      uint8_t* vb = lds + 2 * BLOCK + kbuf;
+      bool found = false;
+      for (int i = threadIdx.x; i < BLOCK / 16; i += 256) {
+        const uint4 v = *reinterpret_cast<const uint4*>(vb + 16 * i);
+        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          found |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
+      }
+      if (__syncthreads_or(found)) {
+        if (!bad)
+          for (int d = threadIdx.x; d < D; d += 256) bad_s[d] = 0x7fffffff;
+        bad = true;
+        __syncthreads();
+        for (int i = threadIdx.x; i < BLOCK / 2; i += 256) {
+          const int r = i / D, d = i % D;
+          uint16_t* p = (uint16_t*)(vb + r * ROW + 16 * ((uint32_t)(d / 8) ^ fa_swz<D>(r)) + 2 * (d % 8));
+          if ((*p & 0x7f80) == 0x7f80) {
+            *p = 0;
+            atomicMin(&bad_s[d], blk * kFaKeys + r);
+          }
+        }
+        __syncthreads();
+      }
+    }
+    // O stays in AGPRs up to the rescale: without this the rescale's copies
+    // out of them were made for every block, rescaled or not
+#pragma unroll
+    for (int d = 0; d < ND; ++d) asm volatile("" : "+a"(o[d]));
+    q35_u32x4 kf[5], vf[2][ND], ph[2];
+    auto readk = [&](int x) {
+      kf[x % 5] = *reinterpret_cast<const q35_u32x4*>(lds + ka[x >> 1] + (BLOCK / 2) * (x & 1));
+    };
+    if constexpr (NEXT) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) readk(x);
+      Q35_PIN();
+    }
+    if (blk * kFaKeys + kFaKeys > least) {
+      mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = blk * kFaKeys + 32 * t + 8 * (r >> 2) + 4 * kh + (r & 3);
+          if (key >= limit) sc[t][r] = -INFINITY;
+          mx = fmaxf(mx, sc[t][r]);
+        }
+    }
+    mx = half_max(mx);
+    if (__ballot(mx > m + 8.f)) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d) asm volatile("" : "+a"(o[d]));
+      const float mn = fmaxf(m, mx);
+      const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= corr;
+      if (__ballot(m != -INFINITY)) {  // else O is still zero
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= corr;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) asm volatile("" : "+a"(o[d]));
+      }
+      m = mn;
+    }
+    // A row without any key so far keeps m = -inf: subtract 0 then.
+    const float ms = m == -INFINITY ? 0.f : m;
+
+    float l1 = 0.f;
+    auto ex = [&](int z) {  // exponential of element z
+      const float p = __builtin_amdgcn_exp2f(sc[z >> 4][z & 15] - ms);
+      sc[z >> 4][z & 15] = p;
+      if (z & 1) l1 += p;
+      else l += p;
+    };
+    auto pack = [&](int kk, int e) {  // P of elements 2 e, 2 e + 1 of k step kk
+      ph[kk & 1][e] = pack_bf2(sc[kk >> 1][8 * (kk & 1) + 2 * e], sc[kk >> 1][8 * (kk & 1) + 2 * e + 1]);
+    };
+    auto readv = [&](int kk, int d) {
+      const uint2 x = lds_read_tr16(lds + va[0][d] + 16 * ROW * kk), y = lds_read_tr16(lds + va[1][d] + 16 * ROW * kk);
+      vf[kk & 1][d] = q35_u32x4{x.x, x.y, y.x, y.y};
+    };
+    if constexpr (NEXT) {
+      constexpr int NS = 2 * KS, EX0 = NS >= 32 ? 12 : 0, PER = NS >= 16 ? 1 : 2;
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        if (x < 2) {
+          q35_f32x16 zero;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+          sn[x] = mfma32(kf[x], qf[0], zero);
+        } else {
+          sn[x & 1] = mfma32(kf[x % 5], qf[x >> 1], sn[x & 1]);
+        }
+        if (x + 4 < NS) readk(x + 4);
+        // every other slot: the texture unit takes a 1 KiB copy in 16 cycles
+        if ((x & 1) == 0 && x < 2 * NC) copy(Kh, kbuf, min(blk + 2, b1 - 1), x >> 1);
+        else if ((x & 1) == 0 && x < 4 * NC) copy(Vh, vbuf, blk + 1, (x >> 1) - NC);
+#pragma unroll
+        for (int z = PER * (x - EX0); z < PER * (x - EX0 + 1); ++z)
+          if (z >= 0 && z < 16) ex(z);
+        if (x >= NS - ND) readv(0, x - (NS - ND));
+        if (NS >= 32 && x >= NS - 4) pack(0, x - (NS - 4));
+        Q35_PIN();
+      }
+      if constexpr (NS < 32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pack(0, e);
+      }
+    } else {
+#pragma unroll
+      for (int d = 0; d < ND; ++d) readv(0, d);
+#pragma unroll
+      for (int z = 0; z < 16; ++z) ex(z);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pack(0, e);
+      Q35_PIN();
+    }
+    if constexpr (NEXT) mx = -INFINITY;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+#pragma unroll
+      for (int y = 0; y < ND; ++y) {
+        o[y] = mfma32(vf[kk & 1][y], ph[kk & 1], o[y]);
+        if (kk < 3) {
+          readv(kk + 1, y);
+          if (kk < 2) {
+#pragma unroll
+            for (int z = 8 * y / ND; z < 8 * (y + 1) / ND; ++z) ex(16 + 8 * kk + z);
+          }
+#pragma unroll
+          for (int e = 4 * y / ND; e < 4 * (y + 1) / ND; ++e) pack(kk + 1, e);
+        }
+        if (NEXT && kk >= 2) {
+#pragma unroll
+          for (int z = 16 * (kk - 2) + 16 * y / ND; z < 16 * (kk - 2) + 16 * (y + 1) / ND; ++z) {
+            const float t = sn[z >> 4][z & 15] * c2;  // into the half of sc that P no longer needs
+            sc[z >> 4][z & 15] = t;
+            mx = fmaxf(mx, t);
+          }
+        }
+        Q35_PIN();
+      }
+    }
+    l += l1;
+    if constexpr (NEXT) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) ka[s] ^= (uint32_t)BLOCK;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) va[u][d] ^= (uint32_t)BLOCK;
+      wait_vm<0>();
+      __syncthreads();
+    }
+  };
+  for (int blk = b0; blk + 1 < b1; ++blk) block(blk, FaTag<true>{});
+  block(b1 - 1, FaTag<false>{});
+
+  l = half_sum(l);
+  if (bad) {  // dims 32 d + 8 u + 4 kh + e of the lane's row
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (bad_s[32 * d + 8 * (r >> 2) + 4 * kh + (r & 3)] < limit) o[d][r] = __builtin_nanf("");
+  }
+  if (nsplit > 1) {
+    // This split's record: O relative to m, not yet divided by l, in register
+    // order (quad u of dim tile d: 64 lanes x 16 bytes), then (m, l) per row.
+    float* rec = a.part + ((((size_t)bh * a.tiles + tile) * a.splits + split) * kFaWaves + w) * F::REC;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<float4*>(rec + ((d * 4 + u) * 64 + lane) * 4) =
+            make_float4(o[d][4 * u], o[d][4 * u + 1], o[d][4 * u + 2], o[d][4 * u + 3]);
+    if (kh == 0) *reinterpret_cast<float2*>(rec + 32 * D + 2 * l32) = make_float2(m, l);
+    return;
+  }
+  const float inv = limit ? 1.0f / l : 0.f;  // a row without keys is zero
+  if (rw + l32 < a.R) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<uint2*>(orow + 32 * d + 8 * u + 4 * kh) =
+            make_uint2(pack_bf2(o[d][4 * u] * inv, o[d][4 * u + 1] * inv),
+                       pack_bf2(o[d][4 * u + 2] * inv, o[d][4 * u + 3] * inv));
+  }
+}
+
+// Merge of the split records of the tiles with more than one: one workgroup per
+// wave record (32 rows), O = sum_s O_s 2^{m_s - M} / sum_s l_s 2^{m_s - M}, M =
+// max_s m_s. Thread (lane, wave) adds quads in the records' own order.
+template <int D>
+__global__ __launch_bounds__(256) void kvq_fa_merge(const FaArgs a) {
+  using F = FaShape<D>;
+  constexpr int NQ = D / 8;  // quads of a record (64 lanes x 4 floats each)
+  __shared__ float f_s[kFaMaxSplits][32], inv_s[32];
+  const int t = threadIdx.x, lane = t & 63;
+  const int w = blockIdx.x & (kFaWaves - 1), tile = blockIdx.x / kFaWaves, bh = blockIdx.y;
+  const int b = bh / a.KVH, kvh = bh % a.KVH;
+  const int r0 = tile * kFaRows, rw = r0 + 32 * w;
+  const long long start = fa_start(a, b);
+  const int n_keys = fa_limit(a, start, min(r0 + kFaRows, a.R) - 1);
+  const int nblk = (n_keys + kFaKeys - 1) / kFaKeys;
+  if (nblk == 0 || rw >= a.R) return;  // whole workgroup
+  const int sb = fa_range(a, nblk), nsplit = (nblk + sb - 1) / sb;
+  if (nsplit <= 1) return;
+  const size_t rs = (size_t)kFaWaves * F::REC;
+  const float* rec0 = a.part + (((size_t)bh * a.tiles + tile) * a.splits * kFaWaves + w) * F::REC;
+  if (t < 32) {
+    float mx = -INFINITY, lt = 0.f;
+    for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, rec0[s * rs + 32 * D + 2 * t]);
+    const float ms = mx == -INFINITY ? 0.f : mx;
+    for (int s = 0; s < nsplit; ++s) {
+      const float2 ml = *reinterpret_cast<const float2*>(rec0 + s * rs + 32 * D + 2 * t);
+      const float f = __builtin_amdgcn_exp2f(ml.x - ms);  // 0 where the row saw no key
+      f_s[s][t] = f;
+      lt = fmaf(ml.y, f, lt);
+    }
+    inv_s[t] = fa_limit(a, start, min(rw + t, a.R - 1)) ? 1.0f / lt : 0.f;
+  }
+  __syncthreads();
+  const int l32 = lane & 31, kh = lane >> 5;
+  constexpr int PER = NQ / 4;
+  float4 acc[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < nsplit; ++s) {
+    const float f = f_s[s][l32];
+    const float* rec = rec0 + s * rs + ((size_t)(t >> 6) * PER * 64 + lane) * 4;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(rec + i * 256);
+      acc[i].x = fmaf(x.x, f, acc[i].x); acc[i].y = fmaf(x.y, f, acc[i].y);
+      acc[i].z = fmaf(x.z, f, acc[i].z); acc[i].w = fmaf(x.w, f, acc[i].w);
+    }
+  }
+  const int row = rw + l32;
+  if (row >= a.R) return;
+  const float inv = inv_s[l32];
+  const int tok = (int)((unsigned)row / (unsigned)a.G), head = kvh * a.G + (row - tok * a.G);
+  uint16_t* orow = a.out + (((size_t)b * a.L + tok) * a.QH + head) * D + 4 * kh;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)  // quad q: dims 8 q + 4 kh ..
+    *reinterpret_cast<uint2*>(orow + 8 * ((t >> 6) * PER + i)) =
+        make_uint2(pack_bf2(acc[i].x * inv, acc[i].y * inv), pack_bf2(acc[i].z * inv, acc[i].w * inv));
+}
+
+struct FaPlan {
+  int tiles, splits;
+  long long part, kv;  // floats of the records and of K or V as bf16
+};
+FaPlan fa_plan(int B, int QH, int KVH, int L, int D, int C) {
+  FaPlan p;
+  const long long rows = (long long)(QH / KVH) * L;
+  p.tiles = (int)((rows + kFaRows - 1) / kFaRows);
+  const long long wgs = (long long)p.tiles * B * KVH, nblk = (C + kFaKeys - 1) / kFaKeys;
+  long long s = 256 / wgs;
+  s = s < 1 ? 1 : s > kFaMaxSplits ? kFaMaxSplits : s;
+  p.splits = (int)(s < (nblk + 1) / 2 ? s : (nblk + 1) / 2);
+  if (p.splits < 1) p.splits = 1;
+  p.part = p.splits > 1 ? wgs * p.splits * kFaWaves * 32 * (D + 2) : 0;
+  p.kv = (long long)B * KVH * C * D / 2;
+  return p;
+}
+
+}  // namespace
+
+long long kvq_prompt_workspace(int B, int QH, int KVH, int L, int D, int C) {
+  const FaPlan p = fa_plan(B, QH, KVH, L, D, C);
+  return 2 * p.kv + p.part;
+}
+
+int kvq_prompt(const void* q, const void* kq, const void* vq, const void* kp, const void* vp, const long long* len,
+               int n_len, long long offset, float scale, void* out, float* workspace, int B, int QH, int KVH, int L,
+               int D, int bits, int C, hipStream_t stream) {
+  const FaPlan p = fa_plan(B, QH, KVH, L, D, C);
+  uint16_t *K = (uint16_t*)workspace, *V = (uint16_t*)(workspace + p.kv);
+  // all rows that any token may see; with the lengths on the device, those it does
+  const int n = len ? C : (int)(offset + L);
+  const long long rows = (long long)B * KVH * n, wgs = (long long)p.tiles * p.splits * B * KVH;
+  Q35_CHECK_ARG(rows < (1ll << 31) && wgs < (1ll << 31) && (long long)B * KVH < 65536);
+  Q35_CHECK_ARG(len || (offset >= 0 && offset + L <= C));
+  const dim3 rgrid((unsigned)((rows + 15) / 16), 2);
+#define Q35_READ(E, BITS)                                                                                             \
+  kvq_read<E, BITS><<<rgrid, 256, 0, stream>>>((const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,            \
+                                               (const uint32_t*)vp, K, V, 0, n, C, C, (unsigned)rows, len, n_len,       \
+                                               offset + L - 1, KVH)
+  if (bits == 4) {
+    if (D == 256) Q35_READ(16, 4); else if (D == 128) Q35_READ(8, 4); else Q35_READ(4, 4);
+  } else {
+    if (D == 256) Q35_READ(16, 8); else if (D == 128) Q35_READ(8, 8); else Q35_READ(4, 8);
+  }
+#undef Q35_READ
+  const FaArgs a{(const uint16_t*)q, K, V, len, n_len, offset, scale, (uint16_t*)out, workspace + 2 * p.kv, QH, KVH, L,
+                 C, C, QH / KVH, QH / KVH * L, p.tiles, p.splits, B * KVH};
+  const dim3 mgrid((unsigned)(p.tiles * kFaWaves), (unsigned)(B * KVH));
+#define Q35_FA(DD)                                                              \
+  do {                                                                          \
+    kvq_fa<DD><<<(unsigned)wgs, kFaWaves * 64, 0, stream>>>(a);                 \
+    if (p.splits > 1) kvq_fa_merge<DD><<<mgrid, 256, 0, stream>>>(a);           \
+  } while (0)
+  if (D == 256) Q35_FA(256); else if (D == 128) Q35_FA(128); else Q35_FA(64);
+#undef Q35_FA
+  return q35_last_error();
+}
