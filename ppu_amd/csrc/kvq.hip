@@ -767,8 +767,8 @@ int q35_kv_dequantize(const void* kq, const void* vq, const void* kp, const void
   const dim3 grid((unsigned)((rows + 15) / 16), 2);
 #define Q35_CALL(E, BITS)                                                                                          \
   kvq_read<E, BITS><<<grid, 256, 0, stream>>>((const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,          \
-                                              (const uint32_t*)vp, (uint16_t*)k, (uint16_t*)v, start, L, L,         \
-                                              capacity, (unsigned)rows, nullptr, 0, 0, KVH)
+                                              (const uint32_t*)vp, (uint16_t*)k, (uint16_t*)v, start, L, capacity,  \
+                                              (unsigned)rows)
   Q35_KVQ_BY_D(Q35_CALL);
 #undef Q35_CALL
   return q35_last_error();

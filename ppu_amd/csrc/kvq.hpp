@@ -33,25 +33,11 @@ Q35_DEV long long kvq_start(const KvqArgs& a, int b) {
   return (a.len ? a.len[a.n_len > 1 ? b : 0] : 0) + a.offset;
 }
 
-// ---------------------------------------------------------------- read back
-// The same 16 lanes a row: bf16(fma(code, step, low)), one rounding. Rows start ..
-// start + L - 1 of every head go to rows of `stride` a head; with a length on
-// the device only the rows that a sequence's last token sees.
+// The values of run c of a row: src its codes, ps the row's first param, groups C
+// apart.
 template <int E, int BITS>
-__global__ __launch_bounds__(256) void kvq_read(const uint8_t* __restrict__ kq, const uint8_t* __restrict__ vq,
-                                                const uint32_t* __restrict__ kp, const uint32_t* __restrict__ vp,
-                                                uint16_t* __restrict__ k, uint16_t* __restrict__ v, int start,
-                                                int L, int stride, int C, unsigned rows, const long long* len,
-                                                int n_len, long long last, int KVH) {
-  constexpr int NG = E / 4, RB = 2 * E * BITS;
-  const unsigned row = blockIdx.x * 16u + (threadIdx.x >> 4);
-  if (row >= rows) return;
-  const int c = threadIdx.x & 15;
-  const unsigned bh = row / (unsigned)L, at = row % (unsigned)L, pos = start + at;
-  if (len && (long long)pos > len[n_len > 1 ? bh / (unsigned)KVH : 0] + last) return;
-  const bool values = blockIdx.y != 0;
-  const uint8_t* src = (values ? vq : kq) + ((size_t)bh * C + pos) * RB + c * (E * BITS / 8);
-  const uint32_t* ps = (values ? vp : kp) + (size_t)bh * NG * C + pos;
+Q35_DEV void kvq_run(const uint8_t* src, const uint32_t* ps, int C, bool values, int c, float (&x)[E]) {
+  constexpr int NG = E / 4;
   uint32_t w[(E * BITS + 31) / 32];
   if constexpr (E * BITS == 16) w[0] = *reinterpret_cast<const uint16_t*>(src);
   else if constexpr (E * BITS == 32) w[0] = *reinterpret_cast<const uint32_t*>(src);
@@ -65,16 +51,32 @@ __global__ __launch_bounds__(256) void kvq_read(const uint8_t* __restrict__ kq, 
   uint32_t p[NG];
 #pragma unroll
   for (int g = 0; g < NG; ++g) p[g] = ps[(size_t)(values ? g : c * E / 64) * C];
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    x[e] = fmaf((float)kvq_code(w[e * BITS / 32], e % (32 / BITS), BITS), bf_lo(p[e / 4]), bf_hi(p[e / 4]));
+}
+
+// ---------------------------------------------------------------- read back
+// The same 16 lanes a row: bf16(fma(code, step, low)), one rounding.
+template <int E, int BITS>
+__global__ __launch_bounds__(256) void kvq_read(const uint8_t* __restrict__ kq, const uint8_t* __restrict__ vq,
+                                                const uint32_t* __restrict__ kp, const uint32_t* __restrict__ vp,
+                                                uint16_t* __restrict__ k, uint16_t* __restrict__ v, int start,
+                                                int L, int C, unsigned rows) {
+  constexpr int NG = E / 4, RB = 2 * E * BITS;
+  const unsigned row = blockIdx.x * 16u + (threadIdx.x >> 4);
+  if (row >= rows) return;
+  const int c = threadIdx.x & 15;
+  const unsigned bh = row / (unsigned)L, pos = start + row % (unsigned)L;
+  const bool values = blockIdx.y != 0;
+  const uint8_t* src = (values ? vq : kq) + ((size_t)bh * C + pos) * RB + c * (E * BITS / 8);
+  const uint32_t* ps = (values ? vp : kp) + (size_t)bh * NG * C + pos;
+  float x[E];
+  kvq_run<E, BITS>(src, ps, C, values, c, x);
   uint32_t o[E / 2];
 #pragma unroll
-  for (int e = 0; e < E; e += 2) {
-    const uint32_t pw = p[e / 4];
-    const float st = bf_lo(pw), lw = bf_hi(pw);
-    const float a = fmaf((float)kvq_code(w[e * BITS / 32], e % (32 / BITS), BITS), st, lw);
-    const float d = fmaf((float)kvq_code(w[e * BITS / 32], e % (32 / BITS) + 1, BITS), st, lw);
-    o[e / 2] = pack_bf2(a, d);
-  }
-  uint16_t* dst = (values ? v : k) + ((size_t)bh * stride + at) * (16 * E) + E * c;
+  for (int e = 0; e < E / 2; ++e) o[e] = pack_bf2(x[2 * e], x[2 * e + 1]);
+  uint16_t* dst = (values ? v : k) + (size_t)row * (16 * E) + E * c;
   if constexpr (E == 4) {
     *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
   } else {

@@ -1,12 +1,15 @@
 // Causal GQA attention of many query rows over the K/V cache in 4 or 8 bits: the
-// cache's values as bf16 in a workspace, one pass over them (kvq_read), and
-// flash attention on the matrix cores over those.
+// cache's values in a workspace, unpacked once, and flash attention on the matrix
+// cores over those.
 //
 // A row tile of 128 rows reads every key once, so a prompt of n rows would
 // unpack a cache n / 128 times inside the attention; unpacked once, its blocks
-// go from memory straight into LDS. The values are rounded to bf16 as a bf16
-// cache holds them, a 2^-8 error at most against a 4-bit step of a fifteenth of
-// the group's range.
+// go from memory straight into LDS. The values are held in 16 bits as fp16 times
+// one power of two per head that brings the greatest of them (by the params,
+// over the keys that are seen) to 2^14: 11 significant bits down to 2^-28 of it,
+// 2^-12 off at most (bf16 would be 2^-8, more than an 8-bit cache's own step).
+// Queries are exact in fp16 times a power of two of their row, but for values
+// below 2^-21 of its greatest.
 #include "kvq.hpp"
 
 namespace {
@@ -22,6 +25,118 @@ constexpr int kFaKeys = 64;       // keys per block
 constexpr int kFaWaves = 4;
 constexpr int kFaRows = 32 * kFaWaves;  // query rows per tile
 constexpr int kFaMaxSplits = 64;
+constexpr int kFaRanges = 64;     // partial maxima of a head's keys or values
+constexpr int kFaSelf = 4096;     // up to this capacity every unpacking workgroup finds the maximum itself
+
+typedef _Float16 q35_f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 q35_f16x8 __attribute__((ext_vector_type(8)));
+Q35_DEV uint32_t pack_h2(float lo, float hi) {
+  const q35_f32x2 v = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, q35_f16x2));
+}
+Q35_DEV q35_f32x16 mfma32h(const q35_u32x4 a, const q35_u32x4 b, q35_f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_f16x8, a), __builtin_bit_cast(q35_f16x8, b), c,
+                                                0, 0, 0);
+}
+// 2^e for -126 <= e <= 127; the e that brings x > 0 to [2^14, 2^15) by 2^e.
+Q35_DEV float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+Q35_DEV int fa_shift(float x) {
+  if (!(x > 0.f)) return 0;
+  const int e = 14 - (ilogbf(x));
+  return e < -113 ? -113 : e > 126 ? 126 : e;
+}
+
+struct UnpackArgs {
+  const uint8_t *kq, *vq;
+  const uint32_t *kp, *vp;
+  const long long* len;
+  int n_len;
+  long long offset;  // of the last token: it sees positions up to len + offset
+  uint16_t *k, *v;
+  float *ranges, *scales;  // [B * KVH, 2, kFaRanges], [B * KVH, 2]
+  int KVH, n, C;
+};
+// Rows of a head that are seen.
+Q35_DEV int unpack_rows(const UnpackArgs& a, int bh) {
+  if (!a.len) return a.n;
+  const long long last = a.len[a.n_len > 1 ? bh / a.KVH : 0] + a.offset;
+  return (int)(last < 0 ? 0 : last >= a.n ? a.n : last + 1);
+}
+// The greatest finite magnitude of the groups that thread t of `threads` takes
+// of a head's first n rows.
+template <int NG, int BITS>
+Q35_DEV float fa_greatest(const uint32_t* p, int n, int C, int t, int threads) {
+  constexpr float T = BITS == 4 ? 15.f : 255.f;
+  float m = 0.f;
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+    for (int i = 4 * t; i < n; i += 4 * threads) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p + (size_t)g * C + i);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float y = fmaxf(fabsf(bf_hi(w[e])), fabsf(fmaf(T, bf_lo(w[e]), bf_hi(w[e]))));
+        if (i + e < n && y < INFINITY) m = fmaxf(m, y);
+      }
+    }
+  return m;
+}
+Q35_DEV float fa_block_max(float m, float* red) {  // of 256 threads
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// Partial maxima of long caches, grid (kFaRanges, keys and values, heads).
+template <int NG, int BITS>
+__global__ __launch_bounds__(256) void kvq_ranges(const UnpackArgs a) {
+  __shared__ float red[4];
+  const int bh = blockIdx.z;
+  const uint32_t* p = (blockIdx.y ? a.vp : a.kp) + (size_t)bh * NG * a.C;
+  const float m = fa_block_max(
+      fa_greatest<NG, BITS>(p, unpack_rows(a, bh), a.C, blockIdx.x * 256 + threadIdx.x, 256 * kFaRanges), red);
+  if (threadIdx.x == 0) a.ranges[(bh * 2 + blockIdx.y) * kFaRanges + blockIdx.x] = m;
+}
+
+// 64 rows a workgroup, 16 lanes a row; grid (blocks, keys and values, heads).
+template <int E, int BITS>
+__global__ __launch_bounds__(256) void kvq_unpack(const UnpackArgs a) {
+  constexpr int NG = E / 4, RB = 2 * E * BITS;
+  __shared__ float red[4];
+  const int bh = blockIdx.z, n = unpack_rows(a, bh), values = blockIdx.y, t = threadIdx.x, c = t & 15;
+  if (blockIdx.x > 0 && (int)blockIdx.x * kFaKeys >= n) return;
+  const uint32_t* p = (values ? a.vp : a.kp) + (size_t)bh * NG * a.C;
+  float m;
+  if (a.ranges) {
+    m = t < kFaRanges ? a.ranges[(bh * 2 + values) * kFaRanges + t] : 0.f;
+  } else {
+    m = fa_greatest<NG, BITS>(p, n, a.C, t, 256);
+  }
+  const int shift = fa_shift(fa_block_max(m, red));
+  const float up = exp2_int(shift);
+  if (blockIdx.x == 0 && t == 0) a.scales[bh * 2 + values] = exp2_int(-shift);
+  const uint8_t* src = (values ? a.vq : a.kq) + (size_t)bh * a.C * RB;
+  uint16_t* dst = (values ? a.v : a.k) + (size_t)bh * a.C * (16 * E);
+#pragma unroll
+  for (int j = 0; j < kFaKeys / 16; ++j) {
+    const int r = blockIdx.x * kFaKeys + 16 * j + (t >> 4);
+    if (r >= n) return;
+    float x[E];
+    kvq_run<E, BITS>(src + (size_t)r * RB + c * (E * BITS / 8), p + r, a.C, values, c, x);
+    uint32_t o[E / 2];
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) o[e] = pack_h2(x[2 * e] * up, x[2 * e + 1] * up);
+    uint16_t* d = dst + (size_t)r * (16 * E) + E * c;
+    if constexpr (E == 4) {
+      *reinterpret_cast<uint2*>(d) = make_uint2(o[0], o[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E / 8; ++i)
+        *reinterpret_cast<uint4*>(d + 8 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    }
+  }
+}
 
 template <int D>
 struct FaShape {
@@ -47,14 +162,15 @@ Q35_DEV uint32_t fa_swz(uint32_t r) {
 }
 
 struct FaArgs {
-  const uint16_t *q, *K, *V;  // K, V [B * KVH, stride, D]
+  const uint16_t *q, *K, *V;  // K, V [B * KVH, C, D] fp16
+  const float* scales;        // [B * KVH, 2]: the values are these times them
   const long long* len;
   int n_len;
   long long offset;
   float scale;
   uint16_t* out;
   float* part;
-  int QH, KVH, L, C, stride, G, R, tiles, splits, bhs;
+  int QH, KVH, L, C, G, R, tiles, splits, bhs;
 };
 Q35_DEV long long fa_start(const FaArgs& a, int b) { return (a.len ? a.len[a.n_len > 1 ? b : 0] : 0) + a.offset; }
 // Keys that row r sees.
@@ -71,13 +187,13 @@ template <bool V> struct FaTag { static constexpr bool value = V; };
 // ------------------------------------------------- attention of many rows
 // Products are transposed: a wave owns 32 query rows (row = token x head of one
 // KV head, so any head grouping fills its tiles) as the COLUMNS of every
-// v_mfma_f32_32x32x16_bf16,
+// v_mfma_f32_32x32x16_f16,
 //   S^T = K Q^T  (A = 32 keys x 16 dims from LDS, B = Q^T held in registers),
 //   O^T += V^T P^T  (A = 32 dims x 16 keys from LDS, B = P^T),
 // so a lane holds one query row: the softmax needs no cross-lane step but one
 // exchange between lanes l and l ^ 32 per block, and the C layout of S^T is,
 // with the 16 keys of a k step taken in the order {0-3, 8-11 | 4-7, 12-15},
-// already the B operand of O^T: P, rounded to bf16, never leaves the registers.
+// already the B operand of O^T: P, rounded to fp16, never leaves the registers.
 // V rows reach the A operand through the transpose read ds_read_b64_tr_b16:
 // within a 16-lane group, lane 4 e + q points at row e, column 4 q and lane i
 // receives the 4 rows of column i.
@@ -90,7 +206,8 @@ template <bool V> struct FaTag { static constexpr bool value = V; };
 // the scale and row maximum of block j + 1.
 //
 // The running maximum m (in units of log2) moves only when a row's block maximum
-// passes it by 8: P stays below 2^8 and O is rescaled a few times per row.
+// passes it by 8, so O is rescaled a few times per row; P is 2^(s - m + 7), below
+// 2^15, with 11 bits down to 2^-21 of the weight at m.
 //
 // Keys past a tile's last one are clamped to it on load and, like every key
 // past a row's own end, masked to -inf in S. In blocks where some row's end
@@ -126,8 +243,8 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
     return;
   }
   const int b1 = nblk - (nsplit - 1 - split) * sb, b0 = split ? b1 - sb : 0;
-  const uint8_t* Kh = (const uint8_t*)(a.K + (size_t)bh * a.stride * D);
-  const uint8_t* Vh = (const uint8_t*)(a.V + (size_t)bh * a.stride * D);
+  const uint8_t* Kh = (const uint8_t*)(a.K + (size_t)bh * a.C * D);
+  const uint8_t* Vh = (const uint8_t*)(a.V + (size_t)bh * a.C * D);
 
   // ---- copies: wave w takes 1 KiB pieces w + 4 i of each block
   const uint32_t cr = (1024u / ROW) * w + lane / F::CPR, cstep = 4u * (1024u / ROW);  // row of copy i: cr + cstep i
@@ -158,17 +275,30 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
     }
   }
 
-  // ---- Q: column l32 of the B operand, dims 16 s + 8 kh ..
+  // ---- Q: column l32 of the B operand, dims 16 s + 8 kh .., in fp16 with the
+  // row's greatest brought to [2^14, 2^15)
   q35_u32x4 qf[KS];
+  float c2 = a.scale * 1.4426950408889634f * a.scales[2 * bh];
   {
     const uint16_t* qp = a.q + (((size_t)b * a.QH + head) * a.L + tok) * D + 8 * kh;
+    float top = 0.f;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const q35_u32x4*>(qp + 16 * s);
+    for (int s = 0; s < KS; ++s) {
+      qf[s] = *reinterpret_cast<const q35_u32x4*>(qp + 16 * s);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(bf_lo(qf[s][e])), fabsf(bf_hi(qf[s][e]))));
+    }
+    const int shift = fa_shift(half_max(top));
+    const float up = exp2_int(shift);
+    c2 *= exp2_int(-shift);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qf[s][e] = pack_h2(bf_lo(qf[s][e]) * up, bf_hi(qf[s][e]) * up);
   }
   const int limit = fa_limit(a, start, row);
   const int least = fa_limit(a, start, min(rw, a.R - 1));     // of the wave's rows
   const int least_wg = fa_limit(a, start, r0);                // of the workgroup's
-  const float c2 = a.scale * 1.4426950408889634f;
   bool bad = false;
 
   q35_f32x16 o[ND], sc[2], sn[2];
@@ -193,7 +323,7 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
     for (int r = 0; r < 16; ++r) sn[t][r] = 0.f;
 #pragma unroll
   for (int x = 0; x < 2 * KS; ++x)
-    sn[x & 1] = mfma32(*reinterpret_cast<const q35_u32x4*>(lds + ka[x >> 1] + (BLOCK / 2) * (x & 1)), qf[x >> 1], sn[x & 1]);
+    sn[x & 1] = mfma32h(*reinterpret_cast<const q35_u32x4*>(lds + ka[x >> 1] + (BLOCK / 2) * (x & 1)), qf[x >> 1], sn[x & 1]);
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -220,7 +350,7 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
         const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          found |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
+          found |= (x[e] & 0x7c00u) == 0x7c00u || (x[e] & 0x7c000000u) == 0x7c000000u;
       }
       if (__syncthreads_or(found)) {
         if (!bad)
@@ -230,7 +360,7 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
         for (int i = threadIdx.x; i < BLOCK / 2; i += 256) {
           const int r = i / D, d = i % D;
           uint16_t* p = (uint16_t*)(vb + r * ROW + 16 * ((uint32_t)(d / 8) ^ fa_swz<D>(r)) + 2 * (d % 8));
-          if ((*p & 0x7f80) == 0x7f80) {
+          if ((*p & 0x7c00) == 0x7c00) {
             *p = 0;
             atomicMin(&bad_s[d], blk * kFaKeys + r);
           }
@@ -280,7 +410,7 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
       m = mn;
     }
     // A row without any key so far keeps m = -inf: subtract 0 then.
-    const float ms = m == -INFINITY ? 0.f : m;
+    const float ms = m == -INFINITY ? 0.f : m - 7.f;
 
     float l1 = 0.f;
     auto ex = [&](int z) {  // exponential of element z
@@ -290,7 +420,7 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
       else l += p;
     };
     auto pack = [&](int kk, int e) {  // P of elements 2 e, 2 e + 1 of k step kk
-      ph[kk & 1][e] = pack_bf2(sc[kk >> 1][8 * (kk & 1) + 2 * e], sc[kk >> 1][8 * (kk & 1) + 2 * e + 1]);
+      ph[kk & 1][e] = pack_h2(sc[kk >> 1][8 * (kk & 1) + 2 * e], sc[kk >> 1][8 * (kk & 1) + 2 * e + 1]);
     };
     auto readv = [&](int kk, int d) {
       const uint2 x = lds_read_tr16(lds + va[0][d] + 16 * ROW * kk), y = lds_read_tr16(lds + va[1][d] + 16 * ROW * kk);
@@ -304,9 +434,9 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
           q35_f32x16 zero;
 #pragma unroll
           for (int r = 0; r < 16; ++r) zero[r] = 0.f;
-          sn[x] = mfma32(kf[x], qf[0], zero);
+          sn[x] = mfma32h(kf[x], qf[0], zero);
         } else {
-          sn[x & 1] = mfma32(kf[x % 5], qf[x >> 1], sn[x & 1]);
+          sn[x & 1] = mfma32h(kf[x % 5], qf[x >> 1], sn[x & 1]);
         }
         if (x + 4 < NS) readk(x + 4);
         // every other slot: the texture unit takes a 1 KiB copy in 16 cycles
@@ -337,7 +467,7 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
     for (int kk = 0; kk < 4; ++kk) {
 #pragma unroll
       for (int y = 0; y < ND; ++y) {
-        o[y] = mfma32(vf[kk & 1][y], ph[kk & 1], o[y]);
+        o[y] = mfma32h(vf[kk & 1][y], ph[kk & 1], o[y]);
         if (kk < 3) {
           readv(kk + 1, y);
           if (kk < 2) {
@@ -394,7 +524,7 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
     if (kh == 0) *reinterpret_cast<float2*>(rec + 32 * D + 2 * l32) = make_float2(m, l);
     return;
   }
-  const float inv = limit ? 1.0f / l : 0.f;  // a row without keys is zero
+  const float inv = limit ? a.scales[2 * bh + 1] / l : 0.f;  // a row without keys is zero
   if (rw + l32 < a.R) {
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -436,7 +566,7 @@ __global__ __launch_bounds__(256) void kvq_fa_merge(const FaArgs a) {
       f_s[s][t] = f;
       lt = fmaf(ml.y, f, lt);
     }
-    inv_s[t] = fa_limit(a, start, min(rw + t, a.R - 1)) ? 1.0f / lt : 0.f;
+    inv_s[t] = fa_limit(a, start, min(rw + t, a.R - 1)) ? a.scales[2 * bh + 1] / lt : 0.f;
   }
   __syncthreads();
   const int l32 = lane & 31, kh = lane >> 5;
@@ -467,7 +597,7 @@ __global__ __launch_bounds__(256) void kvq_fa_merge(const FaArgs a) {
 
 struct FaPlan {
   int tiles, splits;
-  long long part, kv;  // floats of the records and of K or V as bf16
+  long long part, kv, scales;  // floats of the records, of K or V, of the scales and partial maxima
 };
 FaPlan fa_plan(int B, int QH, int KVH, int L, int D, int C) {
   FaPlan p;
@@ -477,9 +607,9 @@ FaPlan fa_plan(int B, int QH, int KVH, int L, int D, int C) {
   long long s = 256 / wgs;
   s = s < 1 ? 1 : s > kFaMaxSplits ? kFaMaxSplits : s;
   p.splits = (int)(s < (nblk + 1) / 2 ? s : (nblk + 1) / 2);
-  if (p.splits < 1) p.splits = 1;
   p.part = p.splits > 1 ? wgs * p.splits * kFaWaves * 32 * (D + 2) : 0;
   p.kv = (long long)B * KVH * C * D / 2;
+  p.scales = ((long long)B * KVH * 2 * (1 + (C > kFaSelf ? kFaRanges : 0)) + 3) / 4 * 4;
   return p;
 }
 
@@ -487,7 +617,7 @@ FaPlan fa_plan(int B, int QH, int KVH, int L, int D, int C) {
 
 long long kvq_prompt_workspace(int B, int QH, int KVH, int L, int D, int C) {
   const FaPlan p = fa_plan(B, QH, KVH, L, D, C);
-  return 2 * p.kv + p.part;
+  return 2 * p.kv + p.part + p.scales;
 }
 
 int kvq_prompt(const void* q, const void* kq, const void* vq, const void* kp, const void* vp, const long long* len,
@@ -495,25 +625,30 @@ int kvq_prompt(const void* q, const void* kq, const void* vq, const void* kp, co
                int D, int bits, int C, hipStream_t stream) {
   const FaPlan p = fa_plan(B, QH, KVH, L, D, C);
   uint16_t *K = (uint16_t*)workspace, *V = (uint16_t*)(workspace + p.kv);
-  // all rows that any token may see; with the lengths on the device, those it does
-  const int n = len ? C : (int)(offset + L);
-  const long long rows = (long long)B * KVH * n, wgs = (long long)p.tiles * p.splits * B * KVH;
-  Q35_CHECK_ARG(rows < (1ll << 31) && wgs < (1ll << 31) && (long long)B * KVH < 65536);
+  float* part = workspace + 2 * p.kv;
+  float* scales = part + p.part;
+  const long long bhs = (long long)B * KVH, wgs = bhs * p.tiles * p.splits;
+  Q35_CHECK_ARG(wgs < (1ll << 31) && bhs < 65536);
   Q35_CHECK_ARG(len || (offset >= 0 && offset + L <= C));
-  const dim3 rgrid((unsigned)((rows + 15) / 16), 2);
-#define Q35_READ(E, BITS)                                                                                             \
-  kvq_read<E, BITS><<<rgrid, 256, 0, stream>>>((const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,            \
-                                               (const uint32_t*)vp, K, V, 0, n, C, C, (unsigned)rows, len, n_len,       \
-                                               offset + L - 1, KVH)
+  // the rows that any token may see; with the lengths on the device, those it does
+  const int n = len ? C : (int)(offset + L);
+  const UnpackArgs u{(const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp, (const uint32_t*)vp, len, n_len,
+                     offset + L - 1, K, V, C > kFaSelf ? scales + 2 * bhs : nullptr, scales, KVH, n, C};
+  const dim3 ugrid((unsigned)((n + kFaKeys - 1) / kFaKeys), 2, (unsigned)bhs);
+#define Q35_UNPACK(E, BITS)                                                                        \
+  do {                                                                                             \
+    if (u.ranges) kvq_ranges<E / 4, BITS><<<dim3(kFaRanges, 2, (unsigned)bhs), 256, 0, stream>>>(u); \
+    kvq_unpack<E, BITS><<<ugrid, 256, 0, stream>>>(u);                                             \
+  } while (0)
   if (bits == 4) {
-    if (D == 256) Q35_READ(16, 4); else if (D == 128) Q35_READ(8, 4); else Q35_READ(4, 4);
+    if (D == 256) Q35_UNPACK(16, 4); else if (D == 128) Q35_UNPACK(8, 4); else Q35_UNPACK(4, 4);
   } else {
-    if (D == 256) Q35_READ(16, 8); else if (D == 128) Q35_READ(8, 8); else Q35_READ(4, 8);
+    if (D == 256) Q35_UNPACK(16, 8); else if (D == 128) Q35_UNPACK(8, 8); else Q35_UNPACK(4, 8);
   }
-#undef Q35_READ
-  const FaArgs a{(const uint16_t*)q, K, V, len, n_len, offset, scale, (uint16_t*)out, workspace + 2 * p.kv, QH, KVH, L,
-                 C, C, QH / KVH, QH / KVH * L, p.tiles, p.splits, B * KVH};
-  const dim3 mgrid((unsigned)(p.tiles * kFaWaves), (unsigned)(B * KVH));
+#undef Q35_UNPACK
+  const FaArgs a{(const uint16_t*)q, K, V, scales, len, n_len, offset, scale, (uint16_t*)out, part, QH, KVH, L,
+                 C, QH / KVH, QH / KVH * L, p.tiles, p.splits, (int)bhs};
+  const dim3 mgrid((unsigned)(p.tiles * kFaWaves), (unsigned)bhs);
 #define Q35_FA(DD)                                                              \
   do {                                                                          \
     kvq_fa<DD><<<(unsigned)wgs, kFaWaves * 64, 0, stream>>>(a);                 \
