@@ -107,6 +107,16 @@ __global__ __launch_bounds__(256) void kvq_unpack(const UnpackArgs a) {
   const int bh = blockIdx.z, n = unpack_rows(a, bh), values = blockIdx.y, t = threadIdx.x, c = t & 15;
   if (blockIdx.x > 0 && (int)blockIdx.x * kFaKeys >= n) return;
   const uint32_t* p = (values ? a.vp : a.kp) + (size_t)bh * NG * a.C;
+  const uint8_t* src = (values ? a.vq : a.kq) + (size_t)bh * a.C * RB + c * (E * BITS / 8);
+  uint16_t* dst = (values ? a.v : a.k) + (size_t)bh * a.C * (16 * E) + E * c;
+  // the workgroup's rows, requested before the maximum is known
+  const int r0 = blockIdx.x * kFaKeys + (t >> 4);
+  float x[kFaKeys / 16][E];
+#pragma unroll
+  for (int j = 0; j < kFaKeys / 16; ++j) {
+    const int r = min(r0 + 16 * j, max(n, 1) - 1);
+    kvq_run<E, BITS>(src + (size_t)r * RB, p + r, a.C, values, c, x[j]);
+  }
   float m;
   if (a.ranges) {
     m = t < kFaRanges ? a.ranges[(bh * 2 + values) * kFaRanges + t] : 0.f;
@@ -116,18 +126,14 @@ __global__ __launch_bounds__(256) void kvq_unpack(const UnpackArgs a) {
   const int shift = fa_shift(fa_block_max(m, red));
   const float up = exp2_int(shift);
   if (blockIdx.x == 0 && t == 0) a.scales[bh * 2 + values] = exp2_int(-shift);
-  const uint8_t* src = (values ? a.vq : a.kq) + (size_t)bh * a.C * RB;
-  uint16_t* dst = (values ? a.v : a.k) + (size_t)bh * a.C * (16 * E);
 #pragma unroll
   for (int j = 0; j < kFaKeys / 16; ++j) {
-    const int r = blockIdx.x * kFaKeys + 16 * j + (t >> 4);
+    const int r = r0 + 16 * j;
     if (r >= n) return;
-    float x[E];
-    kvq_run<E, BITS>(src + (size_t)r * RB + c * (E * BITS / 8), p + r, a.C, values, c, x);
     uint32_t o[E / 2];
 #pragma unroll
-    for (int e = 0; e < E / 2; ++e) o[e] = pack_h2(x[2 * e] * up, x[2 * e + 1] * up);
-    uint16_t* d = dst + (size_t)r * (16 * E) + E * c;
+    for (int e = 0; e < E / 2; ++e) o[e] = pack_h2(x[j][2 * e] * up, x[j][2 * e + 1] * up);
+    uint16_t* d = dst + (size_t)r * (16 * E);
     if constexpr (E == 4) {
       *reinterpret_cast<uint2*>(d) = make_uint2(o[0], o[1]);
     } else {
@@ -145,7 +151,7 @@ struct FaShape {
   static constexpr int CPR = ROW / 16;               // 16-byte chunks of a row
   static constexpr int NC = BLOCK / 1024 / kFaWaves; // a wave's copies of a block
   static constexpr int KS = D / 16, ND = D / 32;     // k steps of S, dim tiles of O
-  static constexpr int REC = 32 * (D + 2);           // floats of a wave's split record
+  static constexpr int REC = 16 * D + 64;            // floats of a wave's split record: O / l as fp16, (m, l)
   static constexpr int WAVES = D > 64 ? 1 : 2;     // waves a SIMD
 };
 
@@ -181,8 +187,6 @@ Q35_DEV int fa_limit(const FaArgs& a, long long start, int r) {
 // Key blocks per range of a tile with nblk of them: over at most `splits`
 // ranges, of at least two blocks.
 Q35_DEV int fa_range(const FaArgs& a, int nblk) { return max((nblk + a.splits - 1) / a.splits, min(nblk, 2)); }
-
-template <bool V> struct FaTag { static constexpr bool value = V; };
 
 // ------------------------------------------------- attention of many rows
 // Products are transposed: a wave owns 32 query rows (row = token x head of one
@@ -256,6 +260,14 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
     dma16(lds0 + to + 4096u * i, base + (size_t)blk * BLOCK, r * ROW + cc[i & 1]);
   };
 
+  // K and V of the first block and K of the second, ahead of Q's preparation
+#pragma unroll
+  for (int i = 0; i < NC; ++i) copy(Kh, 0, b0, i);
+#pragma unroll
+  for (int i = 0; i < NC; ++i) copy(Vh, 2u * BLOCK, b0, i);
+#pragma unroll
+  for (int i = 0; i < NC; ++i) copy(Kh, BLOCK, min(b0 + 1, b1 - 1), i);
+
   // ---- fragment addresses; the buffer is added by ^ BLOCK
   // K: row l32 of a 32-key half (the second half BLOCK / 2 on), chunk 2 s + kh
   uint32_t ka[KS];
@@ -308,14 +320,8 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float m = -INFINITY, l = 0.f, mx = -INFINITY;
 
-  // ---- prologue: K and V of the first block, K of the second; S of the first
-#pragma unroll
-  for (int i = 0; i < NC; ++i) copy(Kh, 0, b0, i);
-#pragma unroll
-  for (int i = 0; i < NC; ++i) copy(Vh, 2u * BLOCK, b0, i);
-#pragma unroll
-  for (int i = 0; i < NC; ++i) copy(Kh, BLOCK, min(b0 + 1, b1 - 1), i);
-  wait_vm<2 * NC>();
+  // ---- S of the first block
+  wait_vm<0>();
   __syncthreads();
 #pragma unroll
   for (int t = 0; t < 2; ++t)
@@ -333,13 +339,13 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
     }
 #pragma unroll
   for (int s = 0; s < KS; ++s) ka[s] ^= (uint32_t)BLOCK;
-  wait_vm<0>();
-  __syncthreads();
+  __syncthreads();  // the loop's first copies go where this K was
 
   // ---- one block: sc holds its scaled scores, mx their maximum over the
-  // lane's keys; ka points at K of the next block, va at V of this one
-  auto block = [&](int blk, auto next_tag) {
-    constexpr bool NEXT = decltype(next_tag)::value;
+  // lane's keys; ka points at K of the next block, va at V of this one. The last
+  // block computes the scores of itself again in place of a next one's: a form
+  // of its own would double the code, which a short range reads cold.
+  for (int blk = b0; blk < b1; ++blk) {
     const uint32_t kbuf = (blk - b0) & 1 ? BLOCK : 0;  // free: this block's K, the last one's V
     const uint32_t vbuf = 2u * BLOCK + (BLOCK - kbuf);
     if (blk * kFaKeys + kFaKeys > least_wg) {  // uniform over the workgroup
@@ -376,11 +382,9 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
     auto readk = [&](int x) {
       kf[x % 5] = *reinterpret_cast<const q35_u32x4*>(lds + ka[x >> 1] + (BLOCK / 2) * (x & 1));
     };
-    if constexpr (NEXT) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) readk(x);
-      Q35_PIN();
-    }
+    for (int x = 0; x < 4; ++x) readk(x);
+    Q35_PIN();
     if (blk * kFaKeys + kFaKeys > least) {
       mx = -INFINITY;
 #pragma unroll
@@ -426,43 +430,33 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
       const uint2 x = lds_read_tr16(lds + va[0][d] + 16 * ROW * kk), y = lds_read_tr16(lds + va[1][d] + 16 * ROW * kk);
       vf[kk & 1][d] = q35_u32x4{x.x, x.y, y.x, y.y};
     };
-    if constexpr (NEXT) {
-      constexpr int NS = 2 * KS, EX0 = NS >= 32 ? 12 : 0, PER = NS >= 16 ? 1 : 2;
+    constexpr int NS = 2 * KS, EX0 = NS >= 32 ? 12 : 0, PER = NS >= 16 ? 1 : 2;
 #pragma unroll
-      for (int x = 0; x < NS; ++x) {
-        if (x < 2) {
-          q35_f32x16 zero;
+    for (int x = 0; x < NS; ++x) {
+      if (x < 2) {
+        q35_f32x16 zero;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) zero[r] = 0.f;
-          sn[x] = mfma32h(kf[x], qf[0], zero);
-        } else {
-          sn[x & 1] = mfma32h(kf[x % 5], qf[x >> 1], sn[x & 1]);
-        }
-        if (x + 4 < NS) readk(x + 4);
-        // every other slot: the texture unit takes a 1 KiB copy in 16 cycles
-        if ((x & 1) == 0 && x < 2 * NC) copy(Kh, kbuf, min(blk + 2, b1 - 1), x >> 1);
-        else if ((x & 1) == 0 && x < 4 * NC) copy(Vh, vbuf, blk + 1, (x >> 1) - NC);
-#pragma unroll
-        for (int z = PER * (x - EX0); z < PER * (x - EX0 + 1); ++z)
-          if (z >= 0 && z < 16) ex(z);
-        if (x >= NS - ND) readv(0, x - (NS - ND));
-        if (NS >= 32 && x >= NS - 4) pack(0, x - (NS - 4));
-        Q35_PIN();
+        for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+        sn[x] = mfma32h(kf[x], qf[0], zero);
+      } else {
+        sn[x & 1] = mfma32h(kf[x % 5], qf[x >> 1], sn[x & 1]);
       }
-      if constexpr (NS < 32) {
+      if (x + 4 < NS) readk(x + 4);
+      // every other slot: the texture unit takes a 1 KiB copy in 16 cycles
+      if ((x & 1) == 0 && x < 2 * NC) copy(Kh, kbuf, min(blk + 2, b1 - 1), x >> 1);
+      else if ((x & 1) == 0 && x < 4 * NC) copy(Vh, vbuf, min(blk + 1, b1 - 1), (x >> 1) - NC);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pack(0, e);
-      }
-    } else {
-#pragma unroll
-      for (int d = 0; d < ND; ++d) readv(0, d);
-#pragma unroll
-      for (int z = 0; z < 16; ++z) ex(z);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pack(0, e);
+      for (int z = PER * (x - EX0); z < PER * (x - EX0 + 1); ++z)
+        if (z >= 0 && z < 16) ex(z);
+      if (x >= NS - ND) readv(0, x - (NS - ND));
+      if (NS >= 32 && x >= NS - 4) pack(0, x - (NS - 4));
       Q35_PIN();
     }
-    if constexpr (NEXT) mx = -INFINITY;
+    if constexpr (NS < 32) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pack(0, e);
+    }
+    mx = -INFINITY;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
 #pragma unroll
@@ -477,7 +471,7 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
 #pragma unroll
           for (int e = 4 * y / ND; e < 4 * (y + 1) / ND; ++e) pack(kk + 1, e);
         }
-        if (NEXT && kk >= 2) {
+        if (kk >= 2) {
 #pragma unroll
           for (int z = 16 * (kk - 2) + 16 * y / ND; z < 16 * (kk - 2) + 16 * (y + 1) / ND; ++z) {
             const float t = sn[z >> 4][z & 15] * c2;  // into the half of sc that P no longer needs
@@ -489,19 +483,15 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
       }
     }
     l += l1;
-    if constexpr (NEXT) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) ka[s] ^= (uint32_t)BLOCK;
+    for (int s = 0; s < KS; ++s) ka[s] ^= (uint32_t)BLOCK;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) va[u][d] ^= (uint32_t)BLOCK;
-      wait_vm<0>();
-      __syncthreads();
-    }
-  };
-  for (int blk = b0; blk + 1 < b1; ++blk) block(blk, FaTag<true>{});
-  block(b1 - 1, FaTag<false>{});
+      for (int d = 0; d < ND; ++d) va[u][d] ^= (uint32_t)BLOCK;
+    wait_vm<0>();
+    __syncthreads();
+  }
 
   l = half_sum(l);
   if (bad) {  // dims 32 d + 8 u + 4 kh + e of the lane's row
@@ -512,16 +502,24 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
         if (bad_s[32 * d + 8 * (r >> 2) + 4 * kh + (r & 3)] < limit) o[d][r] = __builtin_nanf("");
   }
   if (nsplit > 1) {
-    // This split's record: O relative to m, not yet divided by l, in register
-    // order (quad u of dim tile d: 64 lanes x 16 bytes), then (m, l) per row.
+    // This split's record: O / l as fp16 (at most the greatest value, 2^15), in
+    // register order (pair of quads u, u + 1 of dim tile d: 64 lanes x 16
+    // bytes), then (m, l) per row. Halves in place of floats: the records of a
+    // short prompt are most of its traffic.
     float* rec = a.part + ((((size_t)bh * a.tiles + tile) * a.splits + split) * kFaWaves + w) * F::REC;
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        *reinterpret_cast<float4*>(rec + ((d * 4 + u) * 64 + lane) * 4) =
-            make_float4(o[d][4 * u], o[d][4 * u + 1], o[d][4 * u + 2], o[d][4 * u + 3]);
-    if (kh == 0) *reinterpret_cast<float2*>(rec + 32 * D + 2 * l32) = make_float2(m, l);
+      for (int u = 0; u < 2; ++u) {
+        uint4 v;
+        v.x = pack_h2(o[d][8 * u] * inv, o[d][8 * u + 1] * inv);
+        v.y = pack_h2(o[d][8 * u + 2] * inv, o[d][8 * u + 3] * inv);
+        v.z = pack_h2(o[d][8 * u + 4] * inv, o[d][8 * u + 5] * inv);
+        v.w = pack_h2(o[d][8 * u + 6] * inv, o[d][8 * u + 7] * inv);
+        *reinterpret_cast<uint4*>(rec + ((d * 2 + u) * 64 + lane) * 4) = v;
+      }
+    if (kh == 0) *reinterpret_cast<float2*>(rec + 16 * D + 2 * l32) = make_float2(m, l);
     return;
   }
   const float inv = limit ? a.scales[2 * bh + 1] / l : 0.f;  // a row without keys is zero
@@ -537,12 +535,13 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
 }
 
 // Merge of the split records of the tiles with more than one: one workgroup per
-// wave record (32 rows), O = sum_s O_s 2^{m_s - M} / sum_s l_s 2^{m_s - M}, M =
-// max_s m_s. Thread (lane, wave) adds quads in the records' own order.
+// wave record (32 rows), O = sum_s (O / l)_s f_s / sum_s f_s, f_s = l_s 2^{m_s -
+// M}, M = max_s m_s. Thread (lane, wave) adds pairs of quads in the records' own
+// order.
 template <int D>
 __global__ __launch_bounds__(256) void kvq_fa_merge(const FaArgs a) {
   using F = FaShape<D>;
-  constexpr int NQ = D / 8;  // quads of a record (64 lanes x 4 floats each)
+  constexpr int PER = D / 64;  // pairs of quads of a thread
   __shared__ float f_s[kFaMaxSplits][32], inv_s[32];
   const int t = threadIdx.x, lane = t & 63;
   const int w = blockIdx.x & (kFaWaves - 1), tile = blockIdx.x / kFaWaves, bh = blockIdx.y;
@@ -556,32 +555,38 @@ __global__ __launch_bounds__(256) void kvq_fa_merge(const FaArgs a) {
   if (nsplit <= 1) return;
   const size_t rs = (size_t)kFaWaves * F::REC;
   const float* rec0 = a.part + (((size_t)bh * a.tiles + tile) * a.splits * kFaWaves + w) * F::REC;
+  // (m, l) of every split and row
+  __shared__ float2 ml_s[kFaMaxSplits][32];
+  for (int i = t; i < 32 * nsplit; i += 256)
+    ml_s[i >> 5][i & 31] = *reinterpret_cast<const float2*>(rec0 + (i >> 5) * rs + 16 * D + 2 * (i & 31));
+  __syncthreads();
   if (t < 32) {
     float mx = -INFINITY, lt = 0.f;
-    for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, rec0[s * rs + 32 * D + 2 * t]);
+    for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, ml_s[s][t].x);
     const float ms = mx == -INFINITY ? 0.f : mx;
     for (int s = 0; s < nsplit; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(rec0 + s * rs + 32 * D + 2 * t);
-      const float f = __builtin_amdgcn_exp2f(ml.x - ms);  // 0 where the row saw no key
+      const float f = ml_s[s][t].y * __builtin_amdgcn_exp2f(ml_s[s][t].x - ms);  // 0 where the row saw no key
       f_s[s][t] = f;
-      lt = fmaf(ml.y, f, lt);
+      lt += f;
     }
     inv_s[t] = fa_limit(a, start, min(rw + t, a.R - 1)) ? a.scales[2 * bh + 1] / lt : 0.f;
   }
   __syncthreads();
   const int l32 = lane & 31, kh = lane >> 5;
-  constexpr int PER = NQ / 4;
-  float4 acc[PER];
+  float acc[PER][8];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < PER; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[i][e] = 0.f;
+#pragma unroll 4
   for (int s = 0; s < nsplit; ++s) {
     const float f = f_s[s][l32];
     const float* rec = rec0 + s * rs + ((size_t)(t >> 6) * PER * 64 + lane) * 4;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const float4 x = *reinterpret_cast<const float4*>(rec + i * 256);
-      acc[i].x = fmaf(x.x, f, acc[i].x); acc[i].y = fmaf(x.y, f, acc[i].y);
-      acc[i].z = fmaf(x.z, f, acc[i].z); acc[i].w = fmaf(x.w, f, acc[i].w);
+      const q35_f16x8 x = __builtin_bit_cast(q35_f16x8, *reinterpret_cast<const uint4*>(rec + i * 256));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[i][e] = fmaf((float)x[e], f, acc[i][e]);
     }
   }
   const int row = rw + l32;
@@ -590,9 +595,12 @@ __global__ __launch_bounds__(256) void kvq_fa_merge(const FaArgs a) {
   const int tok = (int)((unsigned)row / (unsigned)a.G), head = kvh * a.G + (row - tok * a.G);
   uint16_t* orow = a.out + (((size_t)b * a.L + tok) * a.QH + head) * D + 4 * kh;
 #pragma unroll
-  for (int i = 0; i < PER; ++i)  // quad q: dims 8 q + 4 kh ..
-    *reinterpret_cast<uint2*>(orow + 8 * ((t >> 6) * PER + i)) =
-        make_uint2(pack_bf2(acc[i].x * inv, acc[i].y * inv), pack_bf2(acc[i].z * inv, acc[i].w * inv));
+  for (int i = 0; i < PER; ++i)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)  // quad q: dims 8 q + 4 kh ..
+      *reinterpret_cast<uint2*>(orow + 8 * (2 * ((t >> 6) * PER + i) + u)) =
+          make_uint2(pack_bf2(acc[i][4 * u] * inv, acc[i][4 * u + 1] * inv),
+                     pack_bf2(acc[i][4 * u + 2] * inv, acc[i][4 * u + 3] * inv));
 }
 
 struct FaPlan {
@@ -607,7 +615,7 @@ FaPlan fa_plan(int B, int QH, int KVH, int L, int D, int C) {
   long long s = 256 / wgs;
   s = s < 1 ? 1 : s > kFaMaxSplits ? kFaMaxSplits : s;
   p.splits = (int)(s < (nblk + 1) / 2 ? s : (nblk + 1) / 2);
-  p.part = p.splits > 1 ? wgs * p.splits * kFaWaves * 32 * (D + 2) : 0;
+  p.part = p.splits > 1 ? wgs * p.splits * kFaWaves * (16 * D + 64) : 0;
   p.kv = (long long)B * KVH * C * D / 2;
   p.scales = ((long long)B * KVH * 2 * (1 + (C > kFaSelf ? kFaRanges : 0)) + 3) / 4 * 4;
   return p;
