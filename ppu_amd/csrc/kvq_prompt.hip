@@ -54,6 +54,7 @@ struct UnpackArgs {
   long long offset;  // of the last token: it sees positions up to len + offset
   uint16_t *k, *v;
   float *ranges, *scales;  // [B * KVH, 2, kFaRanges], [B * KVH, 2]
+  int* flags;              // [B * KVH, C / 64 rounded up]: whether a block of values holds an infinity or NaN
   int KVH, n, C;
 };
 // Rows of a head that are seen.
@@ -125,6 +126,15 @@ __global__ __launch_bounds__(256) void kvq_unpack(const UnpackArgs a) {
   }
   const int shift = fa_shift(fa_block_max(m, red));
   const float up = exp2_int(shift);
+  if (values) {
+    float z = 0.f;  // NaN if any value is not finite
+#pragma unroll
+    for (int j = 0; j < kFaKeys / 16; ++j)
+#pragma unroll
+      for (int e = 0; e < E; ++e) z += x[j][e] * 0.f;
+    const bool bad = __syncthreads_or(z != z);
+    if (t == 0) a.flags[(size_t)bh * ((a.C + kFaKeys - 1) / kFaKeys) + blockIdx.x] = bad;
+  }
   if (blockIdx.x == 0 && t == 0) a.scales[bh * 2 + values] = exp2_int(-shift);
 #pragma unroll
   for (int j = 0; j < kFaKeys / 16; ++j) {
@@ -170,6 +180,7 @@ Q35_DEV uint32_t fa_swz(uint32_t r) {
 struct FaArgs {
   const uint16_t *q, *K, *V;  // K, V [B * KVH, C, D] fp16
   const float* scales;        // [B * KVH, 2]: the values are these times them
+  const int* flags;           // [B * KVH, blocks]: V has infinities or NaN
   const long long* len;
   int n_len;
   long long offset;
@@ -215,8 +226,9 @@ Q35_DEV int fa_range(const FaArgs& a, int nblk) { return max((nblk + a.splits - 
 //
 // Keys past a tile's last one are clamped to it on load and, like every key
 // past a row's own end, masked to -inf in S. In blocks where some row's end
-// lies, V's infinities and NaN are taken out and their dims set to NaN at the
-// end for the rows that see them: a weight of zero would not hide them.
+// lies, V's infinities and NaN (the unpacking flags their blocks) are taken out
+// and their dims set to NaN at the end for the rows that see them: a weight of
+// zero would not hide them.
 template <int D>
 __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(const FaArgs a) {
   using F = FaShape<D>;
@@ -311,6 +323,7 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
   const int limit = fa_limit(a, start, row);
   const int least = fa_limit(a, start, min(rw, a.R - 1));     // of the wave's rows
   const int least_wg = fa_limit(a, start, r0);                // of the workgroup's
+  const int* flags = a.flags + (size_t)bh * ((a.C + kFaKeys - 1) / kFaKeys);
   bool bad = false;
 
   q35_f32x16 o[ND], sc[2], sn[2];
@@ -348,31 +361,21 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
   for (int blk = b0; blk < b1; ++blk) {
     const uint32_t kbuf = (blk - b0) & 1 ? BLOCK : 0;  // free: this block's K, the last one's V
     const uint32_t vbuf = 2u * BLOCK + (BLOCK - kbuf);
-    if (blk * kFaKeys + kFaKeys > least_wg) {  // uniform over the workgroup
+    if (blk * kFaKeys + kFaKeys > least_wg && flags[blk]) {  // uniform over the workgroup
       uint8_t* vb = lds + 2 * BLOCK + kbuf;
-      bool found = false;
-      for (int i = threadIdx.x; i < BLOCK / 16; i += 256) {
-        const uint4 v = *reinterpret_cast<const uint4*>(vb + 16 * i);
-        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          found |= (x[e] & 0x7c00u) == 0x7c00u || (x[e] & 0x7c000000u) == 0x7c000000u;
-      }
-      if (__syncthreads_or(found)) {
-        if (!bad)
-          for (int d = threadIdx.x; d < D; d += 256) bad_s[d] = 0x7fffffff;
-        bad = true;
-        __syncthreads();
-        for (int i = threadIdx.x; i < BLOCK / 2; i += 256) {
-          const int r = i / D, d = i % D;
-          uint16_t* p = (uint16_t*)(vb + r * ROW + 16 * ((uint32_t)(d / 8) ^ fa_swz<D>(r)) + 2 * (d % 8));
-          if ((*p & 0x7c00) == 0x7c00) {
-            *p = 0;
-            atomicMin(&bad_s[d], blk * kFaKeys + r);
-          }
+      if (!bad)
+        for (int d = threadIdx.x; d < D; d += 256) bad_s[d] = 0x7fffffff;
+      bad = true;
+      __syncthreads();
+      for (int i = threadIdx.x; i < BLOCK / 2; i += 256) {
+        const int r = i / D, d = i % D;
+        uint16_t* p = (uint16_t*)(vb + r * ROW + 16 * ((uint32_t)(d / 8) ^ fa_swz<D>(r)) + 2 * (d % 8));
+        if ((*p & 0x7c00) == 0x7c00) {
+          *p = 0;
+          atomicMin(&bad_s[d], blk * kFaKeys + r);
         }
-        __syncthreads();
       }
+      __syncthreads();
     }
     // O stays in AGPRs up to the rescale: without this the rescale's copies
     // out of them were made for every block, rescaled or not
@@ -605,7 +608,7 @@ __global__ __launch_bounds__(256) void kvq_fa_merge(const FaArgs a) {
 
 struct FaPlan {
   int tiles, splits;
-  long long part, kv, scales;  // floats of the records, of K or V, of the scales and partial maxima
+  long long part, kv, scales;  // floats of the records, of K or V, of the scales, partial maxima and flags
 };
 FaPlan fa_plan(int B, int QH, int KVH, int L, int D, int C) {
   FaPlan p;
@@ -617,7 +620,7 @@ FaPlan fa_plan(int B, int QH, int KVH, int L, int D, int C) {
   p.splits = (int)(s < (nblk + 1) / 2 ? s : (nblk + 1) / 2);
   p.part = p.splits > 1 ? wgs * p.splits * kFaWaves * (16 * D + 64) : 0;
   p.kv = (long long)B * KVH * C * D / 2;
-  p.scales = ((long long)B * KVH * 2 * (1 + (C > kFaSelf ? kFaRanges : 0)) + 3) / 4 * 4;
+  p.scales = ((long long)B * KVH * (2 + (C > kFaSelf ? 2 * kFaRanges : 0) + nblk) + 3) / 4 * 4;
   return p;
 }
 
@@ -636,12 +639,14 @@ int kvq_prompt(const void* q, const void* kq, const void* vq, const void* kp, co
   float* part = workspace + 2 * p.kv;
   float* scales = part + p.part;
   const long long bhs = (long long)B * KVH, wgs = bhs * p.tiles * p.splits;
+  float* ranges = scales + 2 * bhs;
+  int* flags = (int*)(ranges + (C > kFaSelf ? 2 * kFaRanges * bhs : 0));
   Q35_CHECK_ARG(wgs < (1ll << 31) && bhs < 65536);
   Q35_CHECK_ARG(len || (offset >= 0 && offset + L <= C));
   // the rows that any token may see; with the lengths on the device, those it does
   const int n = len ? C : (int)(offset + L);
   const UnpackArgs u{(const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp, (const uint32_t*)vp, len, n_len,
-                     offset + L - 1, K, V, C > kFaSelf ? scales + 2 * bhs : nullptr, scales, KVH, n, C};
+                     offset + L - 1, K, V, C > kFaSelf ? ranges : nullptr, scales, flags, KVH, n, C};
   const dim3 ugrid((unsigned)((n + kFaKeys - 1) / kFaKeys), 2, (unsigned)bhs);
 #define Q35_UNPACK(E, BITS)                                                                        \
   do {                                                                                             \
@@ -654,7 +659,7 @@ int kvq_prompt(const void* q, const void* kq, const void* vq, const void* kp, co
     if (D == 256) Q35_UNPACK(16, 8); else if (D == 128) Q35_UNPACK(8, 8); else Q35_UNPACK(4, 8);
   }
 #undef Q35_UNPACK
-  const FaArgs a{(const uint16_t*)q, K, V, scales, len, n_len, offset, scale, (uint16_t*)out, part, QH, KVH, L,
+  const FaArgs a{(const uint16_t*)q, K, V, scales, flags, len, n_len, offset, scale, (uint16_t*)out, part, QH, KVH, L,
                  C, QH / KVH, QH / KVH * L, p.tiles, p.splits, (int)bhs};
   const dim3 mgrid((unsigned)(p.tiles * kFaWaves), (unsigned)bhs);
 #define Q35_FA(DD)                                                              \
