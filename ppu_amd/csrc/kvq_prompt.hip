@@ -233,6 +233,7 @@ template <int D>
 __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(const FaArgs a) {
   using F = FaShape<D>;
   constexpr int KS = F::KS, ND = F::ND, NC = F::NC, ROW = F::ROW, BLOCK = F::BLOCK;
+  constexpr int LA = 3;  // K fragments read ahead
   // K buffers at 0 and BLOCK, V buffers at 2 and 3 BLOCK
   __shared__ alignas(1024) uint8_t lds[4 * BLOCK];
   __shared__ int bad_s[D];  // first key of a masked block with a dim's V not finite
@@ -320,6 +321,11 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
 #pragma unroll
       for (int e = 0; e < 4; ++e) qf[s][e] = pack_h2(bf_lo(qf[s][e]) * up, bf_hi(qf[s][e]) * up);
   }
+  // Q stays in AGPRs, which the MFMAs read as they are
+  if constexpr (D == 256) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+a"(qf[s]));
+  }
   const int limit = fa_limit(a, start, row);
   const int least = fa_limit(a, start, min(rw, a.R - 1));     // of the wave's rows
   const int least_wg = fa_limit(a, start, r0);                // of the workgroup's
@@ -381,12 +387,12 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
     // out of them were made for every block, rescaled or not
 #pragma unroll
     for (int d = 0; d < ND; ++d) asm volatile("" : "+a"(o[d]));
-    q35_u32x4 kf[5], vf[2][ND], ph[2];
+    q35_u32x4 kf[LA + 1], vf[2][ND], ph[2];
     auto readk = [&](int x) {
-      kf[x % 5] = *reinterpret_cast<const q35_u32x4*>(lds + ka[x >> 1] + (BLOCK / 2) * (x & 1));
+      kf[x % (LA + 1)] = *reinterpret_cast<const q35_u32x4*>(lds + ka[x >> 1] + (BLOCK / 2) * (x & 1));
     };
 #pragma unroll
-    for (int x = 0; x < 4; ++x) readk(x);
+    for (int x = 0; x < LA; ++x) readk(x);
     Q35_PIN();
     if (blk * kFaKeys + kFaKeys > least) {
       mx = -INFINITY;
@@ -442,9 +448,9 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
         for (int r = 0; r < 16; ++r) zero[r] = 0.f;
         sn[x] = mfma32h(kf[x], qf[0], zero);
       } else {
-        sn[x & 1] = mfma32h(kf[x % 5], qf[x >> 1], sn[x & 1]);
+        sn[x & 1] = mfma32h(kf[x % (LA + 1)], qf[x >> 1], sn[x & 1]);
       }
-      if (x + 4 < NS) readk(x + 4);
+      if (x + LA < NS) readk(x + LA);
       // every other slot: the texture unit takes a 1 KiB copy in 16 cycles
       if ((x & 1) == 0 && x < 2 * NC) copy(Kh, kbuf, min(blk + 2, b1 - 1), x >> 1);
       else if ((x & 1) == 0 && x < 4 * NC) copy(Vh, vbuf, min(blk + 1, b1 - 1), (x >> 1) - NC);
