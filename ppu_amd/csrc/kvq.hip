@@ -271,16 +271,19 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int c16 = lane & 15, kg = lane >> 4, hr = c16 / GT, gl = c16 % GT;
-  // Blocks of the same keys are 8 workgroups apart (one XCD, one L2) and next
-  // in turn.
-  int split = blockIdx.x, blk = 0;
+  // Blocks of the same keys (a unit: split of a KV head) are 8 workgroups apart,
+  // on one XCD and its L2, and next in turn; units go round the XCDs.
+  int split = blockIdx.x, blk = 0, kvh = blockIdx.y, b = blockIdx.z;
   if (a.blocks > 1) {
-    const int x8 = split / 8;
+    const int x8 = (int)blockIdx.x / 8, unit = x8 / a.blocks * 8 + (int)blockIdx.x % 8;
     blk = x8 % a.blocks;
-    split = x8 / a.blocks * 8 + split % 8;
-    if (split >= a.splits) return;
+    const int h = unit / a.splits;
+    split = unit - h * a.splits;
+    b = h / a.KVH;
+    kvh = h - b * a.KVH;
+    if (b >= a.B) return;
   }
-  const int kvh = blockIdx.y, b = blockIdx.z, bh = b * a.KVH + kvh;
+  const int bh = b * a.KVH + kvh;
   const int G = a.G, R = a.R;
 
   __shared__ alignas(1024) uint8_t lds[NW * F::RING + F::QB];
@@ -693,8 +696,16 @@ __global__ __launch_bounds__(256) void kvq_few_merge(const KvqArgs a) {
       make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
 }
 
-// Up to this many query rows of a KV head go to kvq_few.
-constexpr int kKvqFewRows = 64;
+// Whether the rows of a KV head go to kvq_few, which reads and unpacks the keys
+// once per block of rows, or to kvq_prompt, which unpacks them once into memory
+// and has several launches: few rows, or little work in all. Both ways, us (GPU
+// time, 4 bits): 8/2 heads of 256, 32768 tokens: 64 rows 37 / 79, 128 54 / 80,
+// 256 89 / 86, 512 159 / 90; 1024 tokens: 256 rows 15 / 25, 512 27 / 27; 32/8
+// heads of 128, 8 sequences of 32768: 64 rows 231 / 476, 128 448 / 482, 256 816
+// / 613; 14/2 heads of 64, 12 sequences of 1024: 112 rows 13 / 18, 224 20 / 20.
+bool kvq_is_few(long long rows, int B, int KVH, int D, int C) {
+  return rows <= 128 || (double)rows * B * KVH * C * D <= (double)(1 << 28);
+}
 // Rows a block of kvq_few holds: as few columns as the row count needs, as a
 // block's vector work grows with its column tiles.
 int kvq_block_rows(int D, long long rows) {
@@ -778,7 +789,7 @@ long long q35_gqa_attention_kvq_workspace(int B, int QH, int KVH, int L, int D, 
   if (!kvq_shape_ok(B, KVH, L, D, bits, capacity) || QH <= 0 || QH % KVH) return -1;
   const long long rows = (long long)(QH / KVH) * L;
   if ((long long)B * L == 0) return 0;
-  if (rows > kKvqFewRows) return kvq_prompt_workspace(B, QH, KVH, L, D, capacity);
+  if (!kvq_is_few(rows, B, KVH, D, capacity)) return kvq_prompt_workspace(B, QH, KVH, L, D, capacity);
   const int hp = kvq_block_rows(D, rows), blocks = (int)((rows + hp - 1) / hp);
   return (long long)B * KVH * blocks * kvq_splits(B, KVH, blocks, capacity) * hp * (D + 2);
 }
@@ -795,7 +806,7 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
                 q35_aligned16(vp) && q35_aligned16(q) && q35_aligned16(out) && q35_aligned8(gate));
   const long long rows = (long long)(QH / KVH) * L;
   Q35_CHECK_ARG((long long)B * KVH * rows < (1ll << 31));
-  if (rows <= kKvqFewRows) {
+  if (kvq_is_few(rows, B, KVH, D, capacity)) {
     const int hp = kvq_block_rows(D, rows), blocks = (int)((rows + hp - 1) / hp);
     const int splits = kvq_splits(B, KVH, blocks, capacity);
     Q35_CHECK_ARG(B < 65536 && KVH < 65536 && workspace && q35_aligned16(workspace) &&
@@ -803,8 +814,11 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
     const KvqArgs a{(const uint16_t*)q, (const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,
                     (const uint32_t*)vp, (const long long*)len_dev, n_len, offset, (const uint16_t*)gate, gate_stride,
                     scale, (uint16_t*)out, (float*)workspace, QH, KVH, L, capacity, blocks, splits, QH / KVH,
-                    (int)rows};
-    const dim3 grid((unsigned)(blocks == 1 ? splits : (splits + 7) / 8 * 8 * blocks), (unsigned)KVH, (unsigned)B);
+                    (int)rows, B};
+    const long long units = (long long)B * KVH * splits;
+    Q35_CHECK_ARG((units + 7) / 8 * 8 * blocks < (1ll << 31));
+    const dim3 grid = blocks == 1 ? dim3((unsigned)splits, (unsigned)KVH, (unsigned)B)
+                                  : dim3((unsigned)((units + 7) / 8 * 8 * blocks));
     const dim3 mgrid((unsigned)(rows * (D / 64)), (unsigned)KVH, (unsigned)B);
 #define Q35_FEW(DD, HP)                                                            \
   do {                                                                             \

@@ -19,7 +19,7 @@ struct KvqArgs {
   float scale;
   uint16_t* out;
   float* part;
-  int QH, KVH, L, C, blocks, splits, G, R;  // G = QH / KVH, R = G * L
+  int QH, KVH, L, C, blocks, splits, G, R, B;  // G = QH / KVH, R = G * L
 };
 
 // Row r is head r % G of token r / G; a decoded token's rows need no division.

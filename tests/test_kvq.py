@@ -451,6 +451,94 @@ def test_prefill_sizes(gpu, bits, dim, heads, kv_heads, length, start):
     check_attention(got, q, cache, [start], dim**-0.5, prompt=True)
 
 
+def roomy(heads, kv_heads, dim, length, batch=1):
+    """A capacity from which on more than 128 rows of a KV head go over the
+    unpacked cache: rows x batch x KV heads x capacity x dim above 2^28."""
+    capacity = (1 << 28) // (heads // kv_heads * length * batch * kv_heads * dim) + 1
+    return (capacity + 31) // 32 * 32
+
+
+@gpu_test
+@pytest.mark.parametrize("bits,dim", FORMS)
+@pytest.mark.parametrize("heads,kv_heads,length,start", [(8, 2, 33, 0), (8, 2, 65, 63), (3, 1, 70, 100), (12, 1, 50, 7),
+                                                         (2, 2, 400, 1), (5, 1, 129, 319)])
+def test_prefill_many_rows(gpu, bits, dim, heads, kv_heads, length, start):
+    """Row tiles that end inside a token, in the middle of a wave, in several
+    tiles; key ranges of one and several blocks; the rest of the cache NaN."""
+    g = gen(KERNEL_SEED + 916)
+    n, capacity = start + length, roomy(heads, kv_heads, dim, length)
+    k, v = rows(g, 1, kv_heads, n, dim), rows(g, 1, kv_heads, n, dim)
+    cache = cache_of(k, v, bits, capacity, junk=float("nan"))
+    q = torch.randn(1, heads, length, dim, generator=g).to(BF)
+    got = K.gqa_prefill_attention_q(q.to(gpu), to(cache, gpu), dim**-0.5, kv_start=start)
+    check_attention(got, q, cache, [start], dim**-0.5, prompt=True)
+    valid = torch.tensor([start], device=gpu)
+    again = K.gqa_prefill_attention_q(q.to(gpu), to(cache, gpu), dim**-0.5, valid_length=valid, length_is_start=True)
+    assert torch.equal(got, again)
+
+
+@gpu_test
+@pytest.mark.parametrize("bits,dim", [(4, 256), (8, 128), (4, 64)])
+@pytest.mark.parametrize("scale_k,scale_v", [(1e-20, 1e20), (1e4, 1e-30), (2.0**100, 2.0**120)])
+def test_prefill_many_rows_magnitudes(gpu, bits, dim, scale_k, scale_v):
+    """Keys and values far from one, with queries that bring the scores back;
+    one row of queries is zero and one has a value 2^20 above the others."""
+    g = gen(KERNEL_SEED + 917)
+    heads, length = 4, 64
+    capacity = roomy(heads, 1, dim, length)
+    k, v = rows(g, 1, 1, length, dim), rows(g, 1, 1, length, dim)
+    cache = cache_of((k.float() * scale_k).to(BF), (v.float() * scale_v).to(BF), bits, capacity)
+    q = (torch.randn(1, heads, length, dim, generator=g) / scale_k).to(BF)
+    q[0, 1, 5] = 0
+    q[0, 2, 9] *= 2.0**-20
+    q[0, 2, 9, 3] = 1 / scale_k
+    got = K.gqa_prefill_attention_q(q.to(gpu), to(cache, gpu), dim**-0.5).double().cpu() / scale_v
+    # the oracle on the same numbers, brought back in 64 bits
+    kd, vd = values_of(cache)
+    want = ref.attend(q.double() * scale_k, kd / scale_k, vd / scale_v, [0], dim**-0.5)
+    square = ref.attend(q.double() * scale_k, kd / scale_k, (vd / scale_v).square(), [0], dim**-0.5)
+    var = want.square() / 3 + square * (4 / 3)
+    assert torch.isfinite(got).all()
+    assert ((got - want).abs() <= 6 * 2**-8 * var.sqrt()).all()
+
+
+@gpu_test
+@pytest.mark.parametrize("bits,dim,length", [(4, 256, 100), (8, 128, 100), (4, 64, 150)])
+@pytest.mark.parametrize("roomier", [1, 4])
+def test_prefill_batch_many_rows(gpu, bits, dim, length, roomier):
+    """As test_prefill_batch, over the unpacked cache, in short caches and in
+    ones whose greatest values are found by a launch of its own."""
+    g = gen(KERNEL_SEED + 918)
+    capacity = roomier * roomy(4, 2, dim, length, 4)
+    n = 256
+    starts = [0, 77, -length // 2, n - length]
+    cache = cache_of(rows(g, 4, 2, n, dim), rows(g, 4, 2, n, dim), bits, capacity, junk=float("inf"))
+    for b, s in enumerate(starts):
+        cache.key_params[b, :, :, max(s + length, 0) :] = float("nan")
+        cache.value_params[b, :, :, max(s + length, 0) :] = float("nan")
+    # the keys of the last token NaN in one sequence, a group of its values in another
+    cache.key_params[0, :, :, length - 1] = float("nan")
+    cache.value_params[1, :, 0, 77 + length - 1] = float("nan")
+    q = torch.randn(4, 4, length, dim, generator=g).to(BF)
+    valid = torch.tensor([s + length for s in starts], device=gpu)
+    got = K.gqa_prefill_attention_q(q.to(gpu), to(cache, gpu), dim**-0.5, valid_length=valid).cpu()
+    kd, vd = values_of(cache)
+    assert torch.isnan(got[0, -1]).all()
+    want = ref.attend(q[1:2], kd[1:2], vd[1:2], [77], dim**-0.5)[0, -1]
+    assert torch.equal(torch.isnan(got[1, -1]), torch.isnan(want))
+    for b, t in ((0, length - 1), (1, length - 1)):
+        got[b, t] = 0
+    want, square = ref.attend(q, kd, vd, starts, dim**-0.5), ref.attend(q, kd, vd.square(), starts, dim**-0.5)
+    for t in (want, square):
+        t[0, -1] = t[1, -1] = 0
+    assert torch.isfinite(got).all()
+    var = want.square() / 3 + square * (4 / 3)
+    err = (got.double() - want).abs()
+    assert err.square().mean().sqrt() <= 2**-8 * var.mean().sqrt()
+    assert (err <= 6 * 2**-8 * var.sqrt() + 1e-30).all()
+    assert (got[2, : length // 2] == 0).all()
+
+
 @gpu_test
 @pytest.mark.parametrize("bits,dim,length", [(4, 256, 6), (8, 128, 40), (4, 64, 90), (4, 256, 100)])
 @pytest.mark.parametrize("length_is_start", [False, True])
@@ -483,7 +571,8 @@ def test_prefill_long(gpu, bits, dim):
     g = gen(KERNEL_SEED + 912)
     length, start = 67, 5000
     n = start + length
-    cache = cache_of(rows(g, 1, 1, n, dim), rows(g, 1, 1, n, dim), bits, 5088, junk=float("nan"))
+    capacity = max(5088, roomy(4, 1, dim, length))
+    cache = cache_of(rows(g, 1, 1, n, dim), rows(g, 1, 1, n, dim), bits, capacity, junk=float("nan"))
     q = torch.randn(1, 4, length, dim, generator=g).to(BF)
     got = K.gqa_prefill_attention_q(q.to(gpu), to(cache, gpu), dim**-0.5, kv_start=start)
     check_attention(got, q, cache, [start], dim**-0.5, prompt=True)
@@ -560,7 +649,8 @@ def test_two_streams(gpu):
     g = gen(KERNEL_SEED + 915)
     jobs = []
     for heads, kv_heads, dim, length in ((8, 2, 256, 1), (4, 1, 128, 65)):
-        cache = to(cache_of(rows(g, 2, kv_heads, 900, dim), rows(g, 2, kv_heads, 900, dim), 4, 928), gpu)
+        cache = to(cache_of(rows(g, 2, kv_heads, 900, dim), rows(g, 2, kv_heads, 900, dim), 4,
+                            roomy(heads, kv_heads, dim, length, 2) if length > 1 else 928), gpu)
         q = torch.randn(2, heads, length, dim, generator=g).to(BF).to(gpu)
         valid = torch.tensor([900, 411], device=gpu)
         jobs.append((q, cache, valid, dim**-0.5))
