@@ -1321,17 +1321,28 @@ def _kvq_call(name: str, cache: QuantizedKV, operands: tuple, *args) -> None:
     """Launch on the current stream of the cache's GPU, which need not be the
     current GPU; every operand has to be there."""
 
-    device = cache[0].device
-    if device.type != "cuda":
-        raise ValueError(f"fused kernels require GPU tensors: the cache is on {device}")
-    for t in (*cache[1:], *operands):
-        if t is not None and t.device != device:
-            raise ValueError(f"fused kernels require tensors of one GPU: {t.device}, the cache on {device}")
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, _lib.stream(device))
+    kq, vq, kp, vp = cache
+    index = kq.get_device()  # -1 on the CPU
+    if index < 0:
+        raise ValueError(f"fused kernels require GPU tensors: the cache is on {kq.device}")
+    if vq.get_device() != index or kp.get_device() != index or vp.get_device() != index:
+        raise ValueError("fused kernels require the tensors of a cache on one GPU")
+    for t in operands:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"fused kernels require tensors of one GPU: {t.device}, the cache on {kq.device}")
+    # the stream's address alone: a Stream object takes as long as the checks
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = getattr(_lib.load(), name)(*args, stream)
     else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, _lib.stream(device))
+        with torch.cuda.device(index):
+            rc = getattr(_lib.load(), name)(*args, stream)
+    _lib.check(rc, name)
+
+
+@functools.lru_cache(maxsize=256)
+def _kvq_workspace(*sizes: int) -> int:
+    return _lib.load().q35_gqa_attention_kvq_workspace(*sizes)
 
 
 def _kvq_rows(t: torch.Tensor) -> torch.Tensor:
@@ -1386,7 +1397,7 @@ def kv_cache_dequantize(cache: QuantizedKV, length: int, *, start: int = 0) -> t
     if start < 0 or length < 0 or start + length > capacity:
         raise ValueError("rows exceed the quantised cache")
     kq, vq, kp, vp = cache
-    k = torch.empty((batch, kv_heads, length, dim), device=kq.device, dtype=_BF16)
+    k = kp.new_empty((batch, kv_heads, length, dim))
     v = torch.empty_like(k)
     _kvq_call("q35_kv_dequantize", cache, (), kq.data_ptr(), vq.data_ptr(), kp.data_ptr(), vp.data_ptr(),
               k.data_ptr(), v.data_ptr(), start, batch, kv_heads, length, dim, bits, capacity)
@@ -1399,9 +1410,9 @@ def _kvq_attention(q, cache, layout, lengths, offset, scale, gate):
     n_len = _kvq_positions(lengths, batch, "valid_length")
     if q.data_ptr() % 16:
         q = q.clone()
-    out = torch.empty((batch, length, heads * dim), device=q.device, dtype=_BF16)
-    floats = _lib.load().q35_gqa_attention_kvq_workspace(batch, heads, kv_heads, length, dim, bits, capacity)
-    ws = torch.empty(floats, device=q.device, dtype=torch.float32) if floats > 0 else None
+    out = q.new_empty((batch, length, heads * dim))
+    floats = _kvq_workspace(batch, heads, kv_heads, length, dim, bits, capacity)
+    ws = q.new_empty(2 * floats) if floats > 0 else None  # bf16: two to a float
     kq, vq, kp, vp = cache
     _kvq_call("q35_gqa_attention_kvq", cache, (q, lengths, gate), q.data_ptr(), kq.data_ptr(), vq.data_ptr(),
               kp.data_ptr(), vp.data_ptr(), _lib.ptr(lengths), n_len, offset, _lib.ptr(gate),
