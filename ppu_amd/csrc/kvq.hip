@@ -174,15 +174,14 @@ __global__ __launch_bounds__(256) void kvq_write(const KvqSrc ks, const KvqSrc v
 // column is a pair (query row, group): the 16 columns are HP rows x GT of the
 // NG groups, CT = NG / GT column tiles in all. A lane then needs one step and
 // one low per key, its own group's:
-//   S^T[key, (row, group)] = step (K' Q^T + mid' Q sums), K' = the codes (less
-//     half their range) and Q zero outside the column's group; the groups'
-//     parts are added over GT neighbouring lanes. The MFMA accumulates from -c
-//     sum(q), c the offset of the codes as bf16: 4-bit codes become 16 + code by
-//     one shift and one and-or for two of them (24 is taken off), 8-bit codes
-//     are converted (128 is taken off).
+//   S^T[key, (row, group)] = step (K' Q^T) + low sum(q), K' = the codes and Q
+//     zero outside the column's group; the groups' parts are added over GT
+//     neighbouring lanes. 4-bit codes become 16 + code in bf16 by one shift and
+//     one and-or for two of them, and the MFMA accumulates from -16 sum(q);
+//     8-bit codes are converted.
 //   O^T[dim, (row, group)] += V' A^T, A = p step of the column's group as bf16
 //     hi + lo (error below 2^-16: one bf16 would be off by 2^-8 of the group's
-//     half range, whatever the value), and p mid in fp32 beside it; row c of V'
+//     range, whatever the value), and p low in fp32 beside it; row c of V'
 //     product i is dim (D / 16) c + i of every run, all in group i / 4. The
 //     offset's sum over A is one more product with constant rows.
 // P never leaves its lane: the C layout of S^T (lane: 4 keys of a column) is the
@@ -206,7 +205,7 @@ struct KvqFew {
   static constexpr int STAGE = 1024 * NI;               // keys, values, params (2 NG lines of 128 bytes)
   static constexpr int RING = 2 * STAGE;                // a wave's two tiles
   static constexpr int QB = HP * D * 2;                 // bytes of a block's queries
-  static constexpr float OFF = BITS == 4 ? 24.f : 128.f, HALF = BITS == 4 ? 8.f : 128.f;
+  static constexpr float OFF = BITS == 4 ? 16.f : 0.f;  // of a code's operand
   static constexpr int REC = HP * (D + 2);              // floats of a split's record
   static constexpr int WAVES = BITS == 4 && !(D == 256 && HP > 4) ? 2 : 1;  // waves a SIMD, by registers
   struct Tile {
@@ -400,13 +399,15 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   float qs[CT];
   {
     const uint8_t* qp = q_raw + hr * (2 * D) + 32 * kg;
+    const uint32_t neg = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       q35_u32x4 own[2];
       float sum = 0.f;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const uint4 x = *reinterpret_cast<const uint4*>(qp + 128 * (ct * GT + gl) + 16 * s);
+        uint4 x = *reinterpret_cast<const uint4*>(qp + 128 * (ct * GT + gl) + 16 * s);
+        x.x ^= neg; x.y ^= neg; x.z ^= neg; x.w ^= neg;
         sum += ((bf_lo(x.x) + bf_hi(x.x)) + (bf_lo(x.y) + bf_hi(x.y))) +
                ((bf_lo(x.z) + bf_hi(x.z)) + (bf_lo(x.w) + bf_hi(x.w)));
         own[s] = q35_u32x4{__builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
@@ -421,7 +422,8 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
           for (int e = 0; e < 4; ++e) qf[ct * GT + x][s][e] = gl == x ? own[s][e] : 0u;
     }
   }
-  const float c2 = a.scale * 1.4426950408889634f;
+  // log2 e |scale|, the sign in Q; never 0, which would make NaN of a masked -inf
+  const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.0e-37f);
   const KvqMask cm = kvq_mask();
   q35_f32x4 o[NT], cnt[CT];
   float cs[CT];
@@ -433,14 +435,14 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
     cs[ct] = 0.f;
   }
   float m = -INFINITY, l = 0.f;
-  const uint32_t offs = BITS == 4 ? 0xc1c0c1c0u : 0xc300c300u;  // bf16 -24, -128
+  const uint32_t offs = 0xc180c180u;  // bf16 -16
   const q35_u32x4 ones = {offs, offs, offs, offs};
 
   auto step = [&](const Tile& t, int key0) {
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const float z = -F::OFF * qs[ct];
+      const float z = BITS == 4 ? -F::OFF * qs[ct] : 0.f;
       q35_f32x4 acc[2] = {{z, z, z, z}, {z, z, z, z}};
 #pragma unroll
       for (int x = 0; x < GT; ++x) {
@@ -464,14 +466,13 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
       for (int j = 0; j < 8; ++j) {
         const uint32_t pw = t.kp[j >> 2][ct][j & 3];
         const float st = bf_lo(pw);
-        s[j] = fmaf(st, acc[j >> 2][j & 3], fmaf(fmaf(F::HALF, st, bf_hi(pw)), qs[ct], s[j]));
+        s[j] = fmaf(st, acc[j >> 2][j & 3], fmaf(bf_hi(pw), qs[ct], s[j]));
       }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if constexpr (GT > 1) s[j] += dpp_f<Q35_DPP_QUAD_XOR1>(s[j]);
       if constexpr (GT > 2) s[j] += dpp_f<Q35_DPP_QUAD_XOR2>(s[j]);
-      s[j] *= c2;
     }
     float vs[CT][8], vm[CT][8];
 #pragma unroll
@@ -481,9 +482,8 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
         const uint32_t(&pw)[4] = t.vp[tt][ct];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float st = bf_lo(pw[i]);
-          vs[ct][4 * tt + i] = st;
-          vm[ct][4 * tt + i] = fmaf(F::HALF, st, bf_hi(pw[i]));
+          vs[ct][4 * tt + i] = bf_lo(pw[i]);
+          vm[ct][4 * tt + i] = bf_hi(pw[i]);
         }
       }
     if (key0 + 32 > least) {
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
     float mx = s[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[j]);
-    mx = kvq_col_max(mx);
+    mx = kvq_col_max(mx) * c2;
     if (__ballot(mx > m + 8.f)) {
       const float mn = fmaxf(m, mx);
       const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
     float p[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(s[j] - ms);
+      p[j] = __builtin_amdgcn_exp2f(fmaf(s[j], c2, -ms));
       l += p[j];
     }
     q35_u32x4 af[CT], al[CT];
@@ -535,8 +535,10 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
         cs[ct] = fmaf(p[2 * e], vm[ct][2 * e], cs[ct]);
         cs[ct] = fmaf(p[2 * e + 1], vm[ct][2 * e + 1], cs[ct]);
       }
-      cnt[ct] = mfma16(ones, af[ct], cnt[ct]);
-      cnt[ct] = mfma16(ones, al[ct], cnt[ct]);
+      if constexpr (BITS == 4) {
+        cnt[ct] = mfma16(ones, af[ct], cnt[ct]);
+        cnt[ct] = mfma16(ones, al[ct], cnt[ct]);
+      }
     }
     // Four dims a turn (one group): the hi parts' products, then the lo parts'.
 #pragma unroll
