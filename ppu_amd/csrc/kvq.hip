@@ -176,14 +176,18 @@ __global__ __launch_bounds__(256) void kvq_write(const KvqSrc ks, const KvqSrc v
 // one low per key, its own group's:
 //   S^T[key, (row, group)] = step (K' Q^T) + low sum(q), K' = the codes and Q
 //     zero outside the column's group; the groups' parts are added over GT
-//     neighbouring lanes. 4-bit codes become 16 + code in bf16 by one shift and
-//     one and-or for two of them, and the MFMA accumulates from -16 sum(q);
-//     8-bit codes are converted.
+//     neighbouring lanes. The codes are taken as fp8 as they stand: the byte 0000
+//     cccc is c 2^-9 in e4m3, so two ands and a shift make 8 operands of a word
+//     (of 8-bit codes the two halves, 16 apart). Q times a power of two of its
+//     row (its greatest in [2^7, 2^8)) is the sum of two fp8 values, exact but
+//     for values below 2^-10 of the greatest, which are off by 2^-18 of it.
 //   O^T[dim, (row, group)] += V' A^T, A = p step of the column's group as bf16
 //     hi + lo (error below 2^-16: one bf16 would be off by 2^-8 of the group's
-//     range, whatever the value), and p low in fp32 beside it; row c of V'
-//     product i is dim (D / 16) c + i of every run, all in group i / 4. The
-//     offset's sum over A is one more product with constant rows.
+//     range, whatever the value), and p low in fp32 beside it; V' = 16 + code in
+//     bf16 by one shift and one and-or for two 4-bit codes, 8-bit codes are
+//     converted; row c of V' product i is dim (D / 16) c + i of every run, all
+//     in group i / 4. The offset's sum over A is one more product with constant
+//     rows.
 // P never leaves its lane: the C layout of S^T (lane: 4 keys of a column) is the
 // B operand of O^T when the 32 keys of a step are taken in the order {4 kg .. 4
 // kg + 3, 16 + 4 kg ..}. Codes are exact.
@@ -205,7 +209,6 @@ struct KvqFew {
   static constexpr int STAGE = 1024 * NI;               // keys, values, params (2 NG lines of 128 bytes)
   static constexpr int RING = 2 * STAGE;                // a wave's two tiles
   static constexpr int QB = HP * D * 2;                 // bytes of a block's queries
-  static constexpr float OFF = BITS == 4 ? 16.f : 0.f;  // of a code's operand
   static constexpr int REC = HP * (D + 2);              // floats of a split's record
   static constexpr int WAVES = BITS == 4 && !(D == 256 && HP > 4) ? 2 : 1;  // waves a SIMD, by registers
   struct Tile {
@@ -257,6 +260,20 @@ Q35_DEV float kvq_xor16_sum(float v) {
 Q35_DEV float kvq_col_max(float v) { return half_max(kvq_xor16_max(v)); }
 Q35_DEV float kvq_col_sum(float v) { return half_sum(kvq_xor16_sum(v)); }
 
+// Four values as fp8 (e4m3) bytes; byte i back.
+Q35_DEV uint32_t kvq_fp8(const float (&y)[4]) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
+}
+Q35_DEV float kvq_from_fp8(uint32_t w, int i) {
+  return i == 0   ? __builtin_amdgcn_cvt_f32_fp8((int)w, 0)
+         : i == 1 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 1)
+         : i == 2 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 2)
+                  : __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+}
+Q35_DEV q35_f32x4 mfma8(const q35_u32x2 a, const q35_u32x2 b, q35_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(__builtin_bit_cast(long, a), __builtin_bit_cast(long, b), c, 0, 0, 0);
+}
 Q35_DEV q35_f32x4 mfma16(const q35_u32x4 a, const q35_u32x4 b, q35_f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_bf16x8, a), __builtin_bit_cast(q35_bf16x8, b),
                                                  c, 0, 0, 0);
@@ -388,42 +405,73 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
     }
   };
 
-  // ---- Q of the lane's row: dims 64 g + 16 kg + 8 s + {i, i + 4} in word i of
-  // step s, zero outside the column's group; the sums over whole groups. The
-  // queries were copied first: they are there when at most the tiles are not.
+  // ---- Q of the lane's row: dims 64 g + 16 kg + 8 h .. + 7 in step (g, h), zero
+  // outside the column's group, in the order of the codes' bytes. The queries
+  // were copied first: they are there when at most the tiles are not.
   if (tile + stride < n_tiles) wait_vm<2 * F::NI>();
   else if (tile < n_tiles) wait_vm<F::NI>();
   else wait_vm<0>();
   __syncthreads();
-  q35_u32x4 qf[NG][2];
-  float qs[CT];
+  constexpr int P = BITS == 4 ? 2 : 4;
+  q35_u32x2 qf[NG][2][P];
+  float qs[CT], back;  // sums over whole groups; what brings S back
   {
     const uint8_t* qp = q_raw + hr * (2 * D) + 32 * kg;
     const uint32_t neg = a.scale < 0.f ? 0x80008000u : 0u;
+    float x[CT][2][8], top = 0.f;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      q35_u32x4 own[2];
       float sum = 0.f;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        uint4 x = *reinterpret_cast<const uint4*>(qp + 128 * (ct * GT + gl) + 16 * s);
-        x.x ^= neg; x.y ^= neg; x.z ^= neg; x.w ^= neg;
-        sum += ((bf_lo(x.x) + bf_hi(x.x)) + (bf_lo(x.y) + bf_hi(x.y))) +
-               ((bf_lo(x.z) + bf_hi(x.z)) + (bf_lo(x.w) + bf_hi(x.w)));
-        own[s] = q35_u32x4{__builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
-                           __builtin_amdgcn_perm(x.w, x.y, 0x05040100u), __builtin_amdgcn_perm(x.w, x.y, 0x07060302u)};
+      for (int h = 0; h < 2; ++h) {
+        uint4 y = *reinterpret_cast<const uint4*>(qp + 128 * (ct * GT + gl) + 16 * h);
+        y.x ^= neg; y.y ^= neg; y.z ^= neg; y.w ^= neg;
+        unpack8(y, x[ct][h]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          sum += x[ct][h][e];
+          top = fmaxf(top, fabsf(x[ct][h][e]));
+        }
       }
       qs[ct] = kvq_col_sum(sum);
+    }
+    top = kvq_col_max(top);
+    if constexpr (GT > 1) top = fmaxf(top, dpp_f<Q35_DPP_QUAD_XOR1>(top));
+    if constexpr (GT > 2) top = fmaxf(top, dpp_f<Q35_DPP_QUAD_XOR2>(top));
+    const int shift = kvq_shift(top, BITS == 4 ? 7 : 3);
+    const float up = exp2_int(shift);
+    back = exp2_int(-shift);
 #pragma unroll
-      for (int x = 0; x < GT; ++x)
+    for (int ct = 0; ct < CT; ++ct) {
+      qs[ct] *= up * (1.0f / 512.0f);
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) qf[ct * GT + x][s][e] = gl == x ? own[s][e] : 0u;
+        for (int n = 0; n < P / 2; ++n) {
+          const float f = n ? 16.f * up : up;
+          q35_u32x2 own[2];
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = x[ct][h][BITS == 4 ? 2 * e + v : 4 * v + e] * f;
+            own[0][v] = kvq_fp8(y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] -= kvq_from_fp8(own[0][v], e);
+            own[1][v] = kvq_fp8(y);
+          }
+#pragma unroll
+          for (int g = 0; g < GT; ++g)
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+              qf[ct * GT + g][h][2 * n][v] = gl == g ? own[0][v] : 0u;
+              qf[ct * GT + g][h][2 * n + 1][v] = gl == g ? own[1][v] : 0u;
+            }
+        }
     }
   }
   // log2 e |scale|, the sign in Q; never 0, which would make NaN of a masked -inf
-  const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.0e-37f);
+  const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f * 512.f * back, 1.0e-37f);
   const KvqMask cm = kvq_mask();
   q35_f32x4 o[NT], cnt[CT];
   float cs[CT];
@@ -442,8 +490,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const float z = BITS == 4 ? -F::OFF * qs[ct] : 0.f;
-      q35_f32x4 acc[2] = {{z, z, z, z}, {z, z, z, z}};
+      q35_f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int x = 0; x < GT; ++x) {
         const int g = ct * GT + x;
@@ -451,15 +498,20 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt) {
-            q35_u32x4 kf;
             if constexpr (BITS == 4) {
               const uint32_t kw = t.k[tt][g][h];
-              kf = q35_u32x4{kvq_pair4<0>(kw, cm), kvq_pair4<1>(kw, cm), kvq_pair4<2>(kw, cm), kvq_pair4<3>(kw, cm)};
+              const q35_u32x2 kf = {kw & 0x0f0f0f0fu, (kw >> 4) & 0x0f0f0f0fu};
+              acc[tt] = mfma8(kf, qf[g][h][0], acc[tt]);
+              acc[tt] = mfma8(kf, qf[g][h][1], acc[tt]);
             } else {
               const uint32_t k0 = t.k[tt][g][2 * h], k1 = t.k[tt][g][2 * h + 1];
-              kf = q35_u32x4{kvq_pair8<0>(k0, k1), kvq_pair8<1>(k0, k1), kvq_pair8<2>(k0, k1), kvq_pair8<3>(k0, k1)};
+              const q35_u32x2 lo = {k0 & 0x0f0f0f0fu, k1 & 0x0f0f0f0fu};
+              const q35_u32x2 hi = {(k0 >> 4) & 0x0f0f0f0fu, (k1 >> 4) & 0x0f0f0f0fu};
+              acc[tt] = mfma8(lo, qf[g][h][0], acc[tt]);
+              acc[tt] = mfma8(lo, qf[g][h][1], acc[tt]);
+              acc[tt] = mfma8(hi, qf[g][h][2], acc[tt]);
+              acc[tt] = mfma8(hi, qf[g][h][3], acc[tt]);
             }
-            acc[tt] = mfma16(kf, qf[g][h], acc[tt]);
           }
       }
 #pragma unroll

@@ -7,6 +7,17 @@ namespace {
 
 Q35_DEV uint32_t kvq_code(uint32_t w, int i, int bits) { return bits == 4 ? (w >> (4 * i)) & 15u : (w >> (8 * i)) & 255u; }
 
+// 2^e for -126 <= e <= 127; the e that brings x > 0 to [2^to, 2^(to + 1)) by 2^e (a
+// bf16 x is below 2^128, and below 2^-112 it is left smaller).
+Q35_DEV float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+Q35_DEV int kvq_shift(float x, int to) {
+  if (!(x > 0.f)) return 0;
+  const int e = to - ilogbf(x);
+  return e < -120 ? -120 : e > 126 ? 126 : e;
+}
+
+typedef uint32_t q35_u32x2 __attribute__((ext_vector_type(2)));
+
 struct KvqArgs {
   const uint16_t* q;
   const uint8_t *kq, *vq;

@@ -38,14 +38,6 @@ Q35_DEV q35_f32x16 mfma32h(const q35_u32x4 a, const q35_u32x4 b, q35_f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_f16x8, a), __builtin_bit_cast(q35_f16x8, b), c,
                                                 0, 0, 0);
 }
-// 2^e for -126 <= e <= 127; the e that brings x > 0 to [2^14, 2^15) by 2^e.
-Q35_DEV float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-Q35_DEV int fa_shift(float x) {
-  if (!(x > 0.f)) return 0;
-  const int e = 14 - (ilogbf(x));
-  return e < -113 ? -113 : e > 126 ? 126 : e;
-}
-
 struct UnpackArgs {
   const uint8_t *kq, *vq;
   const uint32_t *kp, *vp;
@@ -124,7 +116,7 @@ __global__ __launch_bounds__(256) void kvq_unpack(const UnpackArgs a) {
   } else {
     m = fa_greatest<NG, BITS>(p, n, a.C, t, 256);
   }
-  const int shift = fa_shift(fa_block_max(m, red));
+  const int shift = kvq_shift(fa_block_max(m, red), 14);
   const float up = exp2_int(shift);
   if (values) {
     float z = 0.f;  // NaN if any value is not finite
@@ -313,7 +305,7 @@ __global__ __launch_bounds__(kFaWaves * 64, (FaShape<D>::WAVES)) void kvq_fa(con
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(bf_lo(qf[s][e])), fabsf(bf_hi(qf[s][e]))));
     }
-    const int shift = fa_shift(half_max(top));
+    const int shift = kvq_shift(half_max(top), 14);
     const float up = exp2_int(shift);
     c2 *= exp2_int(-shift);
 #pragma unroll
