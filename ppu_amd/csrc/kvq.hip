@@ -224,7 +224,12 @@ Q35_DEV void kvq_copy(uint32_t lds, const uint8_t* p) {
 // The slot of chunk 0 of a key row of RB bytes in LDS; the place of value row r.
 template <int RB>
 Q35_DEV uint32_t kvq_swz(uint32_t row) { return row / (256 / RB) % (RB / 16); }
-Q35_DEV uint32_t kvq_turn(uint32_t r) { return (r & 16) | ((r & 3) << 2) | ((r >> 2) & 3); }
+template <int RB>
+Q35_DEV uint32_t kvq_turn(uint32_t r) {
+  if (RB == 32) return r;
+  if (RB == 64) return (r & 17) | ((r & 6) << 1) | ((r >> 2) & 2);
+  return (r & 16) | ((r & 3) << 2) | ((r >> 2) & 3);
+}
 
 // Two 4-bit codes (nibble i of each half of w) as 16 + code in bf16.
 // One v_and_or_b32 takes its constants from registers, one of them a vector's.
@@ -279,6 +284,38 @@ Q35_DEV q35_f32x4 mfma16(const q35_u32x4 a, const q35_u32x4 b, q35_f32x4 c) {
                                                  c, 0, 0, 0);
 }
 
+// Sequences of unequal lengths share the workgroups of a KV head (at most 64
+// sequences, lane i holds sequence i): sequence i takes s_i = max(1, floor(share
+// p_i / sum p)) of them, p_i its pieces of 128 keys, at numbers first_i .. first_i
+// + s_i - 1, so that every workgroup has about as many pieces: at most share + B
+// in all, those that are left over last in the launch, as a launch's workgroups
+// are dealt to the CUs in order. With splits fixed a sequence, 60000 and 15 x 1000
+// tokens (8 KV heads of 128) took 99 us.
+constexpr int kKvqShared = 64;
+struct KvqShares {
+  long long start;
+  int s, first;
+};
+Q35_DEV KvqShares kvq_shares(const KvqArgs& a, int lane) {
+  KvqShares v;
+  v.start = (lane < a.B ? a.len[lane] : 0) + a.offset;
+  const int p = lane < a.B ? (kvq_limit(a, v.start, a.L - 1) + 127) / 128 : 0;
+  const int total = wave_sum_i32(p);
+  v.s = p ? max(min(min(p, a.share), (int)((float)p * (float)a.share / (float)total)), 1) : 0;
+  int incl = v.s;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(incl, d, 64);
+    if (lane >= d) incl += o;
+  }
+  v.first = incl - v.s;
+  return v;
+}
+Q35_DEV long long kvq_lane64(long long v, int lane) {
+  return (long long)(((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
+                     (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
+}
+
 template <int D, int BITS, int HP>
 __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(const KvqArgs a) {
   using F = KvqFew<D, BITS, HP>;
@@ -299,6 +336,23 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
     kvh = h - b * a.KVH;
     if (b >= a.B) return;
   }
+  int splits = a.splits, rec_at;
+  long long start;
+  if (a.share) {
+    split = (int)blockIdx.x / a.KVH;
+    kvh = (int)blockIdx.x - split * a.KVH;
+    const KvqShares v = kvq_shares(a, lane);
+    const uint64_t mine = __ballot(split >= v.first && split < v.first + v.s);
+    if (!mine) return;
+    b = __ffsll((long long)mine) - 1;
+    rec_at = (a.share + a.B) * kvh + split;
+    split -= __builtin_amdgcn_readlane(v.first, b);
+    splits = __builtin_amdgcn_readlane(v.s, b);
+    start = kvq_lane64(v.start, b);
+  } else {
+    rec_at = ((b * a.KVH + kvh) * a.blocks + blk) * splits + split;
+    start = kvq_start(a, b);
+  }
   const int bh = b * a.KVH + kvh;
   const int G = a.G, R = a.R;
 
@@ -309,7 +363,6 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   const uint32_t ring0 = __builtin_amdgcn_readfirstlane(lds_offset(ring));
 
   // ---- queries of the block into LDS, wave w's share 1 KiB at a time
-  const long long start = kvq_start(a, b);
   const int row0 = blk * HP;
 #pragma unroll
   for (int z = 0; z < (F::QB + 1024 * NW - 1) / (1024 * NW); ++z) {
@@ -324,8 +377,9 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
 
   // ---- a tile: every copy takes 1 KiB in whole rows. Key rows keep their
   // order, chunk c of 16 bytes at slot c ^ swz(row), so the 16 rows of a
-  // fragment read fall on distinct bank groups; value rows sit transposed, 4 x
-  // 4 within 16, so the 4 rows of a read do.
+  // fragment read fall on distinct bank groups. The value rows that a read
+  // takes, 4 apart, are put next to each other, 4 x 4 transposed within 16 (row
+  // r holds token turn(r)), as far as whole 128-byte lines stay together.
   constexpr int RB = F::RB, CPR = RB / 16;
   const uint8_t* K = a.kq + (size_t)bh * a.C * RB;
   const uint8_t* V = a.vq + (size_t)bh * a.C * RB;
@@ -334,7 +388,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   for (int z = 0; z < F::NK; ++z) {
     const uint32_t row = (64 * z + lane) / CPR, slot = lane % CPR;
     k_at[z] = row * RB + 16 * (slot ^ kvq_swz<RB>(row));
-    v_at[z] = kvq_turn(row) * RB + 16 * slot;
+    v_at[z] = kvq_turn<RB>(row) * RB + 16 * slot;
   }
   const uint8_t* p_at;
   {
@@ -354,7 +408,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   const int least = kvq_limit(a, start, kvq_token(a, row0));
   const int n_max = kvq_limit(a, start, kvq_token(a, min(row0 + HP, R) - 1));
   const int n_tiles = (n_max + 31) / 32;
-  const int stride = a.splits * NW;
+  const int stride = splits * NW;
   int tile = split * NW + w;
   if (tile < n_tiles) issue(tile, 0);
   if (tile + stride < n_tiles) issue(tile + stride, 1);
@@ -363,7 +417,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   uint32_t k_rd[2], v_rd, p_rd;
 #pragma unroll
   for (int tt = 0; tt < 2; ++tt) k_rd[tt] = (16 * tt + c16) * RB;
-  v_rd = 1024 * F::NK + kg * RB + F::RUN * c16;  // token 16 tt + 4 kg + j at row 16 tt + 4 j + kg
+  v_rd = 1024 * F::NK + kg * (RB == 32 ? 4 : RB == 64 ? 2 : 1) * RB + F::RUN * c16;
   p_rd = 2048 * F::NK + 128 * gl + 16 * kg;
   auto fetch = [&](Tile& t, int stage) {
     const uint8_t* s = ring + F::STAGE * stage;
@@ -392,7 +446,9 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint8_t* p = s + v_rd + (16 * (j >> 2) + 4 * (j & 3)) * RB;
+      // token 16 tt + 4 kg + i
+      const int i = j & 3, at = RB == 32 ? i : RB == 64 ? 8 * (i >> 1) + (i & 1) : 4 * i;
+      const uint8_t* p = s + v_rd + (16 * (j >> 2) + at) * RB;
       if constexpr (F::RUN == 2) t.v[j][0] = *reinterpret_cast<const uint16_t*>(p);
       else if constexpr (F::RUN == 4) t.v[j][0] = *reinterpret_cast<const uint32_t*>(p);
       else if constexpr (F::RUN == 8) {
@@ -663,7 +719,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
     ml_s[w][hr][1] = l;
   }
   __syncthreads();
-  float* rec = a.part + ((size_t)(bh * a.blocks + blk) * a.splits + split) * F::REC;
+  float* rec = a.part + (size_t)rec_at * F::REC;
   for (int x = threadIdx.x; x < HP * D / 4; x += 256) {
     const int h = x / (D / 4), d = 4 * (x % (D / 4));
     float mm = -INFINITY;
@@ -699,17 +755,26 @@ __global__ __launch_bounds__(256) void kvq_few_merge(const KvqArgs a) {
   // Requested together: a part's records, the thread's split's (m, l) and the
   // length that says which of them were written.
   const float* rec = a.part + (size_t)(bh * a.blocks + blk) * a.splits * REC;
-  const long long start = kvq_start(a, b);
-  const float2 raw = *reinterpret_cast<const float2*>(rec + (size_t)min(t, a.splits - 1) * REC + HP * D + 2 * h);
+  long long start;
+  int splits = a.splits;
+  if (a.share) {
+    const KvqShares v = kvq_shares(a, t & 63);
+    rec = a.part + (size_t)((a.share + a.B) * kvh + __builtin_amdgcn_readlane(v.first, b)) * REC;
+    splits = max(__builtin_amdgcn_readlane(v.s, b), 1);
+    start = kvq_lane64(v.start, b);
+  } else {
+    start = kvq_start(a, b);
+  }
+  const float2 raw = *reinterpret_cast<const float2*>(rec + (size_t)min(t, splits - 1) * REC + HP * D + 2 * h);
   float4 x[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j)
-    x[j] = *reinterpret_cast<const float4*>(rec + (size_t)min(part + 16 * j, a.splits - 1) * REC + h * D + d);
+    x[j] = *reinterpret_cast<const float4*>(rec + (size_t)min(part + 16 * j, splits - 1) * REC + h * D + d);
   const int i = kvq_token(a, r), head = kvh * a.G + (r - i * a.G);
   const uint2 gate = a.gate ? *reinterpret_cast<const uint2*>(a.gate + b * a.gate_stride + (2 * head + 1) * D + d)
                             : make_uint2(0, 0);
   const int n_max = kvq_limit(a, start, kvq_token(a, min(blk * HP + HP, a.R) - 1));
-  const int n = min(a.splits, ((n_max + 31) / 32 + NW - 1) / NW);
+  const int n = min(splits, ((n_max + 31) / 32 + NW - 1) / NW);
   __shared__ float f_s[kKvqSplits], red_s[2][4];
   __shared__ float4 sum_s[16][16];
   const float m = t < n ? raw.x : -INFINITY, l = t < n ? raw.y : 0.f;
@@ -775,6 +840,28 @@ int kvq_splits(int B, int KVH, int blocks, int C) {
   long long s = kKvqTarget / ((long long)B * KVH * blocks);
   s = s < 1 ? 1 : s > kKvqSplits ? kKvqSplits : s;
   return (int)(s < pieces ? s : pieces);
+}
+// How a call's row blocks spread over workgroups, and its workspace.
+struct KvqFewPlan {
+  int hp, blocks, splits, share;
+  long long floats;
+};
+KvqFewPlan kvq_few_plan(int B, int KVH, long long rows, int D, int C, bool lengths) {
+  KvqFewPlan p;
+  p.hp = kvq_block_rows(D, rows);
+  p.blocks = (int)((rows + p.hp - 1) / p.hp);
+  p.splits = kvq_splits(B, KVH, p.blocks, C);
+  // several sequences with lengths of their own and one block: shared
+  p.share = 0;
+  const long long most = (long long)((C + 127) / 128) * B;  // pieces of a KV head
+  if (lengths && B > 1 && B <= kKvqShared && p.blocks == 1) {
+    const int s = kKvqTarget / KVH;
+    p.share = s < 1 ? 1 : s > kKvqSplits ? kKvqSplits : s;
+    if (p.share > most) p.share = (int)most;
+  }
+  const long long fixed = (long long)B * KVH * p.blocks * p.splits, shared = (long long)KVH * (p.share + B);
+  p.floats = (fixed > shared ? fixed : shared) * p.hp * (D + 2);
+  return p;
 }
 
 bool kvq_shape_ok(int B, int KVH, int L, int D, int bits, int C) {
@@ -844,8 +931,7 @@ long long q35_gqa_attention_kvq_workspace(int B, int QH, int KVH, int L, int D, 
   const long long rows = (long long)(QH / KVH) * L;
   if ((long long)B * L == 0) return 0;
   if (!kvq_is_few(rows, B, KVH, D, capacity)) return kvq_prompt_workspace(B, QH, KVH, L, D, capacity);
-  const int hp = kvq_block_rows(D, rows), blocks = (int)((rows + hp - 1) / hp);
-  return (long long)B * KVH * blocks * kvq_splits(B, KVH, blocks, capacity) * hp * (D + 2);
+  return kvq_few_plan(B, KVH, rows, D, capacity, true).floats;
 }
 
 int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const void* kp, const void* vp,
@@ -861,25 +947,24 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
   const long long rows = (long long)(QH / KVH) * L;
   Q35_CHECK_ARG((long long)B * KVH * rows < (1ll << 31));
   if (kvq_is_few(rows, B, KVH, D, capacity)) {
-    const int hp = kvq_block_rows(D, rows), blocks = (int)((rows + hp - 1) / hp);
-    const int splits = kvq_splits(B, KVH, blocks, capacity);
-    Q35_CHECK_ARG(B < 65536 && KVH < 65536 && workspace && q35_aligned16(workspace) &&
-                  workspace_floats >= (long long)B * KVH * splits * blocks * hp * (D + 2));
+    const KvqFewPlan p = kvq_few_plan(B, KVH, rows, D, capacity, n_len > 1);
+    Q35_CHECK_ARG(B < 65536 && KVH < 65536 && workspace && q35_aligned16(workspace) && workspace_floats >= p.floats);
     const KvqArgs a{(const uint16_t*)q, (const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,
                     (const uint32_t*)vp, (const long long*)len_dev, n_len, offset, (const uint16_t*)gate, gate_stride,
-                    scale, (uint16_t*)out, (float*)workspace, QH, KVH, L, capacity, blocks, splits, QH / KVH,
-                    (int)rows, B};
-    const long long units = (long long)B * KVH * splits;
-    Q35_CHECK_ARG((units + 7) / 8 * 8 * blocks < (1ll << 31));
-    const dim3 grid = blocks == 1 ? dim3((unsigned)splits, (unsigned)KVH, (unsigned)B)
-                                  : dim3((unsigned)((units + 7) / 8 * 8 * blocks));
+                    scale, (uint16_t*)out, (float*)workspace, QH, KVH, L, capacity, p.blocks, p.splits,
+                    QH / KVH, (int)rows, B, p.share};
+    const long long units = (long long)B * KVH * p.splits, wgs = (units + 7) / 8 * 8 * p.blocks;
+    Q35_CHECK_ARG(wgs < (1ll << 31));
+    const dim3 grid = p.share ? dim3((unsigned)((p.share + B) * KVH))
+                      : p.blocks == 1 ? dim3((unsigned)p.splits, (unsigned)KVH, (unsigned)B) : dim3((unsigned)wgs);
+    const int most = p.share ? p.share : p.splits, hp = p.hp;  // records of a row
     const dim3 mgrid((unsigned)(rows * (D / 64)), (unsigned)KVH, (unsigned)B);
 #define Q35_FEW(DD, HP)                                                            \
   do {                                                                             \
     if (bits == 4) kvq_few<DD, 4, HP><<<grid, 256, 0, stream>>>(a);                \
     else kvq_few<DD, 8, HP><<<grid, 256, 0, stream>>>(a);                          \
-    if (splits <= 16) kvq_few_merge<DD, HP, 1><<<mgrid, 256, 0, stream>>>(a);      \
-    else if (splits <= 64) kvq_few_merge<DD, HP, 4><<<mgrid, 256, 0, stream>>>(a); \
+    if (most <= 16) kvq_few_merge<DD, HP, 1><<<mgrid, 256, 0, stream>>>(a);      \
+    else if (most <= 64) kvq_few_merge<DD, HP, 4><<<mgrid, 256, 0, stream>>>(a); \
     else kvq_few_merge<DD, HP, 16><<<mgrid, 256, 0, stream>>>(a);                  \
   } while (0)
     if (D == 64) Q35_FEW(64, 16);

@@ -31,6 +31,7 @@ struct KvqArgs {
   uint16_t* out;
   float* part;
   int QH, KVH, L, C, blocks, splits, G, R, B;  // G = QH / KVH, R = G * L
+  int share;  // workgroups that a KV head's sequences share by their lengths; 0: `splits` for each
 };
 
 // Row r is head r % G of token r / G; a decoded token's rows need no division.
