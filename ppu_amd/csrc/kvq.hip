@@ -210,7 +210,7 @@ struct KvqFew {
   static constexpr int RING = 2 * STAGE;                // a wave's two tiles
   static constexpr int QB = HP * D * 2;                 // bytes of a block's queries
   static constexpr int REC = HP * (D + 2);              // floats of a split's record
-  static constexpr int WAVES = BITS == 4 && !(D == 256 && HP > 4) ? 2 : 1;  // waves a SIMD, by registers
+  static constexpr int WAVES = BITS == 4 && !(D == 256 && HP > 8) ? 2 : 1;  // waves a SIMD, by registers
   struct Tile {
     uint32_t k[2][NG][KW], v[8][VR], kp[2][CT][4], vp[2][CT][4];
   };
@@ -419,7 +419,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   for (int tt = 0; tt < 2; ++tt) k_rd[tt] = (16 * tt + c16) * RB;
   v_rd = 1024 * F::NK + kg * (RB == 32 ? 4 : RB == 64 ? 2 : 1) * RB + F::RUN * c16;
   p_rd = 2048 * F::NK + 128 * gl + 16 * kg;
-  auto fetch = [&](Tile& t, int stage) {
+  auto fetch_k = [&](Tile& t, int stage) {
     const uint8_t* s = ring + F::STAGE * stage;
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
@@ -440,10 +440,18 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
       for (int ct = 0; ct < CT; ++ct) {
         const uint4 x = *reinterpret_cast<const uint4*>(s + p_rd + 128 * GT * ct + 64 * tt);
         t.kp[tt][ct][0] = x.x; t.kp[tt][ct][1] = x.y; t.kp[tt][ct][2] = x.z; t.kp[tt][ct][3] = x.w;
+      }
+    }
+  };
+  auto fetch_v = [&](Tile& t, int stage) {
+    const uint8_t* s = ring + F::STAGE * stage;
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
         const uint4 y = *reinterpret_cast<const uint4*>(s + p_rd + 128 * (NG + GT * ct) + 64 * tt);
         t.vp[tt][ct][0] = y.x; t.vp[tt][ct][1] = y.y; t.vp[tt][ct][2] = y.z; t.vp[tt][ct][3] = y.w;
       }
-    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       // token 16 tt + 4 kg + i
@@ -542,7 +550,10 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
   const uint32_t offs = 0xc180c180u;  // bf16 -16
   const q35_u32x4 ones = {offs, offs, offs, offs};
 
-  auto step = [&](const Tile& t, int key0) {
+  auto step = [&](int tile, int stage) {
+    const int key0 = 32 * tile;
+    Tile t;
+    fetch_k(t, stage);
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -582,6 +593,13 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
       if constexpr (GT > 1) s[j] += dpp_f<Q35_DPP_QUAD_XOR1>(s[j]);
       if constexpr (GT > 2) s[j] += dpp_f<Q35_DPP_QUAD_XOR2>(s[j]);
     }
+    // the tile's last reads, and its place takes the copies of the tile after next
+    Q35_PIN();
+    fetch_v(t, stage);
+    wait_lds();
+    Q35_PIN();
+    if (tile + 2 * stride < n_tiles) issue(tile + 2 * stride, stage);
+    Q35_PIN();
     float vs[CT][8], vm[CT][8];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
@@ -675,20 +693,13 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
       for (int i = 0; i < 4; ++i) o[4 * g + i] = mfma16(vf[i], al[g / GT], o[4 * g + i]);
     }
   };
-  // Two tiles in flight: a tile is read into registers whole, then its place
-  // takes the copies of the tile after next, then it is used.
+  // Two tiles in flight.
   for (int stage = 0; tile < n_tiles; stage ^= 1) {
     if (tile + stride < n_tiles) wait_vm<F::NI>();
     else wait_vm<0>();
     asm volatile("" : : : "memory");
     Q35_PIN();
-    Tile t;
-    fetch(t, stage);
-    wait_lds();
-    Q35_PIN();
-    if (tile + 2 * stride < n_tiles) issue(tile + 2 * stride, stage);
-    Q35_PIN();
-    step(t, 32 * tile);
+    step(tile, stage);
     Q35_PIN();
     tile += stride;
   }
@@ -826,11 +837,16 @@ bool kvq_is_few(long long rows, int B, int KVH, int D, int C) {
   return rows <= 128 || (double)rows * B * KVH * C * D <= (double)(1 << 28);
 }
 // Rows a block of kvq_few holds: as few columns as the row count needs, as a
-// block's vector work grows with its column tiles.
-int kvq_block_rows(int D, long long rows) {
+// block's vector work grows with its column tiles. In heads of 256 sixteen rows
+// leave one wave on a SIMD, which 4-bit codes feel until the second reading of
+// the keys costs more. 8 a block / 16, us, 8/2 heads of 256, 4 bits: 12 rows
+// after 1024 tokens 8.9 / 11.4, after 32768 16.5 / 22.9; 64 rows 16.7 / 24.7 and
+// 30 / 37, 6 sequences of 32768 124 / 127; 128 rows there 288 / 233. In 8 bits 12
+// rows 10.1 / 12.3 and 26 / 26, 6 sequences 68 / 58; 64 rows 217 / 149.
+int kvq_block_rows(int D, int bits, long long rows) {
   if (D == 64) return 16;
   if (D == 128) return rows <= 8 ? 8 : 16;
-  return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+  return rows <= 4 ? 4 : rows <= (bits == 4 ? 64 : 8) ? 8 : 16;
 }
 // Splits of every KV head's keys: from the capacity, as the valid length is not
 // known here; up to kKvqTarget workgroups in all.
@@ -846,9 +862,9 @@ struct KvqFewPlan {
   int hp, blocks, splits, share;
   long long floats;
 };
-KvqFewPlan kvq_few_plan(int B, int KVH, long long rows, int D, int C, bool lengths) {
+KvqFewPlan kvq_few_plan(int B, int KVH, long long rows, int D, int bits, int C, bool lengths) {
   KvqFewPlan p;
-  p.hp = kvq_block_rows(D, rows);
+  p.hp = kvq_block_rows(D, bits, rows);
   p.blocks = (int)((rows + p.hp - 1) / p.hp);
   p.splits = kvq_splits(B, KVH, p.blocks, C);
   // several sequences with lengths of their own and one block: shared
@@ -931,7 +947,7 @@ long long q35_gqa_attention_kvq_workspace(int B, int QH, int KVH, int L, int D, 
   const long long rows = (long long)(QH / KVH) * L;
   if ((long long)B * L == 0) return 0;
   if (!kvq_is_few(rows, B, KVH, D, capacity)) return kvq_prompt_workspace(B, QH, KVH, L, D, capacity);
-  return kvq_few_plan(B, KVH, rows, D, capacity, true).floats;
+  return kvq_few_plan(B, KVH, rows, D, bits, capacity, true).floats;
 }
 
 int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const void* kp, const void* vp,
@@ -947,7 +963,7 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
   const long long rows = (long long)(QH / KVH) * L;
   Q35_CHECK_ARG((long long)B * KVH * rows < (1ll << 31));
   if (kvq_is_few(rows, B, KVH, D, capacity)) {
-    const KvqFewPlan p = kvq_few_plan(B, KVH, rows, D, capacity, n_len > 1);
+    const KvqFewPlan p = kvq_few_plan(B, KVH, rows, D, bits, capacity, n_len > 1);
     Q35_CHECK_ARG(B < 65536 && KVH < 65536 && workspace && q35_aligned16(workspace) && workspace_floats >= p.floats);
     const KvqArgs a{(const uint16_t*)q, (const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,
                     (const uint32_t*)vp, (const long long*)len_dev, n_len, offset, (const uint16_t*)gate, gate_stride,
