@@ -180,7 +180,9 @@ __global__ __launch_bounds__(256) void kvq_write(const KvqSrc ks, const KvqSrc v
 //     cccc is c 2^-9 in e4m3, so two ands and a shift make 8 operands of a word
 //     (of 8-bit codes the two halves, 16 apart). Q times a power of two of its
 //     row (its greatest in [2^7, 2^8)) is the sum of two fp8 values, exact but
-//     for values below 2^-10 of the greatest, which are off by 2^-18 of it.
+//     for values below 2^-9 of the greatest, which are off by 2^-17 of it at
+//     most; for the low halves of 8-bit codes it is 2^-4 of that, so 2^-5 and
+//     2^-13, of at most 15 steps where the group has 255.
 //   O^T[dim, (row, group)] += V' A^T, A = p step of the column's group as bf16
 //     hi + lo (error below 2^-16: one bf16 would be off by 2^-8 of the group's
 //     range, whatever the value), and p low in fp32 beside it; V' = 16 + code in
@@ -194,9 +196,8 @@ __global__ __launch_bounds__(256) void kvq_write(const KvqSrc ks, const KvqSrc v
 //
 // The running maximum m (log2 units) moves only when a tile passes it by 8, so O
 // is rescaled a few times a row. Tiles are dealt in turn, so any valid length
-// spreads over all splits, and a wave's first tile does not depend on it: its
-// loads go out before the length arrives. Keys past a row's end are masked in S
-// and their A and mid set to zero, whatever their params hold.
+// spreads over all splits. Keys past a row's end are masked in S and their step
+// and low set to zero, whatever their params hold.
 template <int D, int BITS, int HP>
 struct KvqFew {
   static constexpr int NG = D / 64, GT = NG < 16 / HP ? NG : 16 / HP, CT = NG / GT, NW = 4;
@@ -833,8 +834,9 @@ __global__ __launch_bounds__(256) void kvq_few_merge(const KvqArgs a) {
 // 256 89 / 86, 512 159 / 90; 1024 tokens: 256 rows 15 / 25, 512 27 / 27; 32/8
 // heads of 128, 8 sequences of 32768: 64 rows 231 / 476, 128 448 / 482, 256 816
 // / 613; 14/2 heads of 64, 12 sequences of 1024: 112 rows 13 / 18, 224 20 / 20.
-bool kvq_is_few(long long rows, int B, int KVH, int D, int C) {
-  return rows <= 128 || (double)rows * B * KVH * C * D <= (double)(1 << 28);
+// One query position is always kvq_few's, which alone applies the gate.
+bool kvq_is_few(long long rows, int B, int KVH, int L, int D, int C) {
+  return L == 1 || rows <= 128 || (double)rows * B * KVH * C * D <= (double)(1 << 28);
 }
 // Rows a block of kvq_few holds: as few columns as the row count needs, as a
 // block's vector work grows with its column tiles. In heads of 256 sixteen rows
@@ -946,7 +948,7 @@ long long q35_gqa_attention_kvq_workspace(int B, int QH, int KVH, int L, int D, 
   if (!kvq_shape_ok(B, KVH, L, D, bits, capacity) || QH <= 0 || QH % KVH) return -1;
   const long long rows = (long long)(QH / KVH) * L;
   if ((long long)B * L == 0) return 0;
-  if (!kvq_is_few(rows, B, KVH, D, capacity)) return kvq_prompt_workspace(B, QH, KVH, L, D, capacity);
+  if (!kvq_is_few(rows, B, KVH, L, D, capacity)) return kvq_prompt_workspace(B, QH, KVH, L, D, capacity);
   return kvq_few_plan(B, KVH, rows, D, bits, capacity, true).floats;
 }
 
@@ -962,8 +964,8 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
                 q35_aligned16(vp) && q35_aligned16(q) && q35_aligned16(out) && q35_aligned8(gate));
   const long long rows = (long long)(QH / KVH) * L;
   Q35_CHECK_ARG((long long)B * KVH * rows < (1ll << 31));
-  if (kvq_is_few(rows, B, KVH, D, capacity)) {
-    const KvqFewPlan p = kvq_few_plan(B, KVH, rows, D, bits, capacity, n_len > 1);
+  if (kvq_is_few(rows, B, KVH, L, D, capacity)) {
+    const KvqFewPlan p = kvq_few_plan(B, KVH, rows, D, bits, capacity, len_dev && n_len > 1);
     Q35_CHECK_ARG(B < 65536 && KVH < 65536 && workspace && q35_aligned16(workspace) && workspace_floats >= p.floats);
     const KvqArgs a{(const uint16_t*)q, (const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,
                     (const uint32_t*)vp, (const long long*)len_dev, n_len, offset, (const uint16_t*)gate, gate_stride,

@@ -410,6 +410,63 @@ def test_decode_gate(gpu, bits):
 
 
 @gpu_test
+def test_decode_gate_many_heads(gpu):
+    """More than 128 heads on one KV head in a roomy cache, with a gate: one
+    token is the decode kernel's at any size."""
+    g = gen(KERNEL_SEED + 930)
+    heads, dim, n = 144, 64, 100
+    cache = cache_of(rows(g, 1, 1, n, dim), rows(g, 1, 1, n, dim), 4, roomy(heads, 1, dim, 1), junk=float("nan"))
+    q = torch.randn(1, heads, 1, dim, generator=g).to(BF)
+    packed = (2 * torch.randn(1, 1, 2 * dim * heads, generator=g)).to(BF)
+    got = K.gqa_decode_attention_q(q.to(gpu), to(cache, gpu), torch.tensor(n, device=gpu), dim**-0.5,
+                                   packed_gate=packed.to(gpu))
+    gate = packed.double().unflatten(-1, (heads, 2, dim))[..., 1, :].flatten(2)
+    check_attention(got, q, cache, [n - 1], dim**-0.5, gate=torch.sigmoid(gate))
+
+
+@gpu_test
+@pytest.mark.parametrize("bits,dim", [(4, 256), (8, 128), (4, 64)])
+@pytest.mark.parametrize("scale_q,scale_k,scale_v",
+                         [(1e20, 1e-20, 1e30), (1e-25, 1e25, 1e-12), (2.0**-100, 2.0**100, 1.0)])
+def test_decode_magnitudes(gpu, bits, dim, scale_q, scale_k, scale_v):
+    """Far from 1 each, the scores as ever: no power of two is lost."""
+    g = gen(KERNEL_SEED + 931)
+    n = 301
+    k = (rows(g, 1, 2, n, dim).float() * scale_k).to(BF)
+    v = (rows(g, 1, 2, n, dim).float() * scale_v).to(BF)
+    cache = cache_of(k, v, bits, 320, junk=float("nan"))
+    q = (torch.randn(1, 8, 1, dim, generator=g) * scale_q).to(BF)
+    got = K.gqa_decode_attention_q(q.to(gpu), to(cache, gpu), torch.tensor(n, device=gpu), dim**-0.5)
+    check_attention(got, q, cache, [n - 1], dim**-0.5)
+
+
+@gpu_test
+@pytest.mark.parametrize("bits,dim,length", [(4, 256, 1), (8, 256, 1), (4, 128, 2), (8, 64, 1)])
+@pytest.mark.parametrize("lengths", [[4000, 3, 0, 33, 129, 5, 1, 64, 2], [1, 2500], [700] * 3 + [0] * 5])
+def test_decode_unequal_lengths(gpu, bits, dim, length, lengths):
+    """Sequences that share a KV head's workgroups: one long among short and
+    empty ones."""
+    g = gen(KERNEL_SEED + 932)
+    batch, capacity = len(lengths), 4032
+    cache = cache_of(rows(g, batch, 2, max(lengths), dim), rows(g, batch, 2, max(lengths), dim), bits, capacity)
+    q = torch.randn(batch, 6, length, dim, generator=g).to(BF)
+    got = K.gqa_prefill_attention_q(q.to(gpu), to(cache, gpu), dim**-0.5, valid_length=torch.tensor(lengths, device=gpu))
+    check_attention(got, q, cache, [n - length for n in lengths], dim**-0.5)
+
+
+@gpu_test
+def test_decode_large_batches(gpu):
+    """More sequences than a wave has lanes, lengths from 0 on."""
+    g = gen(KERNEL_SEED + 933)
+    batch, dim = 70, 64
+    lengths = [(7 * i) % 97 for i in range(batch)]
+    cache = cache_of(rows(g, batch, 1, 96, dim), rows(g, batch, 1, 96, dim), 4, 96)
+    q = torch.randn(batch, 3, 1, dim, generator=g).to(BF)
+    got = K.gqa_decode_attention_q(q.to(gpu), to(cache, gpu), torch.tensor(lengths, device=gpu), dim**-0.5)
+    check_attention(got, q, cache, [n - 1 for n in lengths], dim**-0.5)
+
+
+@gpu_test
 @pytest.mark.parametrize("bits,dim", [(4, 256), (8, 256), (4, 128), (8, 64)])
 def test_decode_long(gpu, bits, dim):
     """A long cache: many splits and several tiles of every wave."""
@@ -641,6 +698,63 @@ def test_decode_step_captured(gpu):
         torch.cuda.synchronize()
         assert torch.equal(out, want), f"replay {i}"
     assert int(length[0]) == n0 + 6
+
+
+@gpu_test
+@pytest.mark.parametrize("length,many", [(5, False), (70, True)])
+def test_prompt_captured(gpu, length, many):
+    """Parts of a prompt, written and attended in one graph that is replayed
+    along the cache, with eager calls between: the same bits as eager."""
+    g = gen(KERNEL_SEED + 934)
+    heads, kv_heads, dim, n0, parts = 8, 2, 128, 40, 4
+    capacity = roomy(heads, kv_heads, dim, length) if many else 512
+    n = n0 + parts * length
+    k, v = rows(g, 1, kv_heads, n, dim).to(gpu), rows(g, 1, kv_heads, n, dim).to(gpu)
+    qs = torch.randn(parts, 1, heads, length, dim, generator=g).to(BF).to(gpu)
+    caches = [K.quantized_kv_cache(1, kv_heads, capacity, dim, bits=8, device=gpu) for _ in range(2)]
+    for c in caches:
+        K.kv_cache_quantize(k[:, :, :n0], v[:, :, :n0], c)
+    at = [torch.tensor([n0], device=gpu) for _ in range(2)]
+
+    def step(cache, at, q, kn, vn):
+        K.kv_cache_quantize(kn, vn, cache, cache_start=at)
+        out = K.gqa_prefill_attention_q(q, cache, dim**-0.5, valid_length=at, length_is_start=True)
+        at.add_(length)
+        return out
+
+    q, kn, vn = qs[0].clone(), k[:, :, n0 : n0 + length].clone(), v[:, :, n0 : n0 + length].clone()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(caches[0], at[0].clone(), q, kn, vn)  # the same rows again below
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(caches[0], at[0], q, kn, vn)
+    for i in range(parts):
+        part = slice(n0 + i * length, n0 + (i + 1) * length)
+        for dst, src in ((q, qs[i]), (kn, k[:, :, part]), (vn, v[:, :, part])):
+            dst.copy_(src)
+        graph.replay()
+        want = step(caches[1], at[1], qs[i], k[:, :, part], v[:, :, part])
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), f"replay {i}"
+
+
+@gpu_test
+def test_entry_without_lengths(gpu):
+    """The C entry with no lengths takes their count for nothing."""
+    g = gen(KERNEL_SEED + 935)
+    batch, dim, n = 3, 128, 64
+    cache = cache_of(rows(g, batch, 2, n, dim), rows(g, batch, 2, n, dim), 4, n)
+    q = torch.randn(batch, 4, 1, dim, generator=g).to(BF)
+    c, qd = to(cache, gpu), q.to(gpu)
+    out = torch.empty(batch, 1, 4 * dim, device=gpu, dtype=BF)
+    floats = _lib.load().q35_gqa_attention_kvq_workspace(batch, 4, 2, 1, dim, 4, n)
+    ws = torch.empty(floats, device=gpu)
+    _lib.call("q35_gqa_attention_kvq", qd.data_ptr(), c.keys.data_ptr(), c.values.data_ptr(), c.key_params.data_ptr(),
+              c.value_params.data_ptr(), 0, batch, 40, 0, 0, dim**-0.5, out.data_ptr(), ws.data_ptr(), floats,
+              batch, 4, 2, 1, dim, 4, n, torch.cuda.current_stream().cuda_stream)
+    check_attention(out, q, cache, [40] * batch, dim**-0.5)
 
 
 @gpu_test
