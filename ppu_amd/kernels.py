@@ -1281,29 +1281,37 @@ def quantized_kv_cache(batch: int, kv_heads: int, capacity: int, head_dim: int, 
     return QuantizedKV(*codes, *params)
 
 
-def _kvq_layout(cache: QuantizedKV) -> tuple[int, int, int, int, int]:
-    """Check a cache's form; ``(batch, KV heads, capacity, head dim, bits)``."""
+@functools.lru_cache(maxsize=256)
+def _kvq_form(kq: torch.Size, vq: torch.Size, kp: torch.Size, vp: torch.Size) -> tuple[int, int, int, int, int]:
+    """Check the shapes of a cache (once for each); as ``_kvq_layout``."""
 
-    kq, vq, kp, vp = cache
-    if kq.ndim != 4 or kp.ndim != 5 or vq.shape != kq.shape or vp.shape != kp.shape:
+    if len(kq) != 4 or len(kp) != 5 or vq != kq or vp != kp:
         raise ValueError("quantised cache: codes [B,KVH,C,D*bits/8] and params [B,KVH,D/64,C,2], K as V")
-    if not (kq.dtype == vq.dtype == torch.uint8 and kp.dtype == vp.dtype == _BF16):
-        raise ValueError("quantised cache: uint8 codes and bfloat16 params")
-    batch, kv_heads, capacity, width = kq.shape
-    groups = kp.shape[2]
+    batch, kv_heads, capacity, width = kq
+    groups = kp[2]
     dim = 64 * groups
     bits = width * 8 // dim if dim else 0
     if groups not in (1, 2, 4) or bits not in (4, 8) or width * 8 != dim * bits:
         raise ValueError("a quantised K/V cache has 4 or 8 bits and heads of 64, 128 or 256")
-    if kp.shape != (batch, kv_heads, groups, capacity, 2) or batch == 0 or kv_heads == 0:
+    if tuple(kp) != (batch, kv_heads, groups, capacity, 2) or batch == 0 or kv_heads == 0:
         raise ValueError("quantised cache: codes and params do not match")
     if capacity == 0 or capacity % 32 or capacity * width >= 1 << 31:
         raise ValueError("quantised cache capacity must be a multiple of 32 (and a head's codes below 2 GiB)")
+    return batch, kv_heads, capacity, dim, bits
+
+
+def _kvq_layout(cache: QuantizedKV) -> tuple[int, int, int, int, int]:
+    """Check a cache's form; ``(batch, KV heads, capacity, head dim, bits)``."""
+
+    kq, vq, kp, vp = cache
+    if not (kq.dtype == vq.dtype == torch.uint8 and kp.dtype == vp.dtype == _BF16):
+        raise ValueError("quantised cache: uint8 codes and bfloat16 params")
+    layout = _kvq_form(kq.shape, vq.shape, kp.shape, vp.shape)
     if not (kq.is_contiguous() and vq.is_contiguous() and kp.is_contiguous() and vp.is_contiguous()):
         raise ValueError("quantised cache tensors must be contiguous")
     if (kq.data_ptr() | vq.data_ptr() | kp.data_ptr() | vp.data_ptr()) % 16:
         raise ValueError("quantised cache tensors must be 16-byte aligned")
-    return batch, kv_heads, capacity, dim, bits
+    return layout
 
 
 def _kvq_positions(t: torch.Tensor | None, batch: int, name: str) -> int:
@@ -1406,7 +1414,7 @@ def kv_cache_dequantize(cache: QuantizedKV, length: int, *, start: int = 0) -> t
 
 def _kvq_attention(q, cache, layout, lengths, offset, scale, gate):
     batch, kv_heads, capacity, dim, bits = layout
-    heads, length = q.shape[1], q.shape[2]
+    _, heads, length, _ = q.shape
     n_len = _kvq_positions(lengths, batch, "valid_length")
     if q.data_ptr() % 16:
         q = q.clone()
@@ -1421,13 +1429,16 @@ def _kvq_attention(q, cache, layout, lengths, offset, scale, gate):
     return out
 
 
-def _kvq_query(q: torch.Tensor, layout) -> None:
-    batch, kv_heads, _, dim, _ = layout
-    if q.ndim != 4 or q.shape[0] != batch or q.shape[3] != dim or q.shape[1] == 0 or q.shape[1] % kv_heads:
+def _kvq_query(q: torch.Tensor, layout) -> int:
+    """Check the queries; their tokens."""
+
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != layout[0] or shape[3] != layout[3] or shape[1] == 0 or shape[1] % layout[1]:
         raise ValueError("attention head layout does not match the quantised cache")
     if not q.is_contiguous():
         raise ValueError("attention queries must be contiguous")
     _need_bf16(q)
+    return shape[2]
 
 
 def gqa_decode_attention_q(
@@ -1446,8 +1457,7 @@ def gqa_decode_attention_q(
     bf16, rounded once; zeros for a sequence without valid positions."""
 
     layout = _kvq_layout(cache)
-    _kvq_query(q, layout)
-    if q.shape[2] != 1:
+    if _kvq_query(q, layout) != 1:
         raise ValueError("GQA decode attention expects q[B,H,1,D]")
     if packed_gate is not None:
         width = packed_gate.shape[-1]
@@ -1477,8 +1487,7 @@ def gqa_prefill_attention_q(
     bf16."""
 
     layout = _kvq_layout(cache)
-    _kvq_query(q, layout)
-    capacity, length = layout[2], q.shape[2]
+    capacity, length = layout[2], _kvq_query(q, layout)
     if valid_length is None:
         if length_is_start:
             raise ValueError("length_is_start needs valid_length")
