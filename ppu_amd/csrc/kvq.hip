@@ -850,12 +850,23 @@ int kvq_block_rows(int D, int bits, long long rows) {
   if (D == 128) return rows <= 8 ? 8 : 16;
   return rows <= 4 ? 4 : rows <= (bits == 4 ? 64 : 8) ? 8 : 16;
 }
+// Workgroups of a launch of `units` KV heads x row blocks, up to which their keys
+// are split: one a CU for the long rows of one block, which are bound by memory,
+// and for all of 256 bytes, which leave a SIMD one wave; two a CU for shorter ones
+// and several blocks, and where whole splits would leave a fifth of the CUs idle.
+// 256 / 512, us, one token after 131071: 8/2 heads of 256 20.5 / 22.5 (8 bits 31.0
+// / 36.9), 32/8 heads of 128 in 8 bits 47.9 / 52.2, in 4 bits 35.3 / 33.5, 14/2
+// heads of 64, 8 sequences 51.4 / 40.3; 16 tokens after 32768, 6 sequences, 8/2
+// heads of 256 186 / 124 (8 bits 142 / 149); 1024 was never better.
+int kvq_target(int D, int bits, int blocks, long long units) {
+  const int row = D * bits / 8;
+  return row >= (blocks == 1 ? 128 : 256) && 256 / units * units >= 208 ? 256 : 512;
+}
 // Splits of every KV head's keys: from the capacity, as the valid length is not
-// known here; up to kKvqTarget workgroups in all.
-constexpr int kKvqTarget = 512;
-int kvq_splits(int B, int KVH, int blocks, int C) {
-  const long long pieces = (C + 127) / 128;
-  long long s = kKvqTarget / ((long long)B * KVH * blocks);
+// known here.
+int kvq_splits(int B, int KVH, int blocks, int D, int bits, int C) {
+  const long long pieces = (C + 127) / 128, units = (long long)B * KVH * blocks;
+  long long s = kvq_target(D, bits, blocks, units) / units;
   s = s < 1 ? 1 : s > kKvqSplits ? kKvqSplits : s;
   return (int)(s < pieces ? s : pieces);
 }
@@ -868,12 +879,12 @@ KvqFewPlan kvq_few_plan(int B, int KVH, long long rows, int D, int bits, int C, 
   KvqFewPlan p;
   p.hp = kvq_block_rows(D, bits, rows);
   p.blocks = (int)((rows + p.hp - 1) / p.hp);
-  p.splits = kvq_splits(B, KVH, p.blocks, C);
+  p.splits = kvq_splits(B, KVH, p.blocks, D, bits, C);
   // several sequences with lengths of their own and one block: shared
   p.share = 0;
   const long long most = (long long)((C + 127) / 128) * B;  // pieces of a KV head
   if (lengths && B > 1 && B <= kKvqShared && p.blocks == 1) {
-    const int s = kKvqTarget / KVH;
+    const int s = kvq_target(D, bits, 1, KVH) / KVH;
     p.share = s < 1 ? 1 : s > kKvqSplits ? kKvqSplits : s;
     if (p.share > most) p.share = (int)most;
   }

@@ -26,7 +26,11 @@ constexpr int kFaWaves = 4;
 constexpr int kFaRows = 32 * kFaWaves;  // query rows per tile
 constexpr int kFaMaxSplits = 64;
 constexpr int kFaRanges = 64;     // partial maxima of a head's keys or values
-constexpr int kFaSelf = 4096;     // up to this capacity every unpacking workgroup finds the maximum itself
+// Up to this capacity every unpacking workgroup finds the maximum itself; above,
+// a launch of its own finds partial maxima. Self / launch, us, 8/2 heads of 256: 1000
+// tokens of 1024 33.1 / 35.1, 300 of 2048 38.4 / 38.9, 1000 of 4096 63.9 / 61.8, 300
+// of 8192 64.2 / 57.7.
+constexpr int kFaSelf = 2048;
 
 typedef _Float16 q35_f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 q35_f16x8 __attribute__((ext_vector_type(8)));
@@ -608,6 +612,14 @@ struct FaPlan {
   int tiles, splits;
   long long part, kv, scales;  // floats of the records, of K or V, of the scales, partial maxima and flags
 };
+// Ranges of a tile's keys: up to one workgroup a CU (for heads of 64, two that have
+// four blocks), as each more adds to the merge, and two for up to that many tiles
+// of a long cache, whose causal lengths would leave the early ones' CUs idle.
+// Target 256 / 512, us: 8/2 heads of 256, 1024 tokens 33.1 / 41.4, 1000 after 31768 295
+// / 306, but 3000 tokens (188 tiles) 101 / 75, 4096 (256) 132 / 109, 4096 after 28672
+// 988 / 976; 32/8 of 128, 1024 tokens (256 tiles) 32.6 / 38.9, 1000 after 3096 98.7 /
+// 99.6; 14/2 of 64, 1500 tokens 30.4 / 26.0, 1000 after 31768 235 / 190, 300 after 1748
+// (ranges of two blocks) 19.6 / 22.7.
 FaPlan fa_plan(int B, int QH, int KVH, int L, int D, int C) {
   FaPlan p;
   const long long rows = (long long)(QH / KVH) * L;
@@ -615,7 +627,14 @@ FaPlan fa_plan(int B, int QH, int KVH, int L, int D, int C) {
   const long long wgs = (long long)p.tiles * B * KVH, nblk = (C + kFaKeys - 1) / kFaKeys;
   long long s = 256 / wgs;
   s = s < 1 ? 1 : s > kFaMaxSplits ? kFaMaxSplits : s;
-  p.splits = (int)(s < (nblk + 1) / 2 ? s : (nblk + 1) / 2);
+  s = s < (nblk + 1) / 2 ? s : (nblk + 1) / 2;
+  if (D == 64) {
+    const long long two = 512 / wgs < (nblk + 3) / 4 ? 512 / wgs : (nblk + 3) / 4;
+    s = two > s ? (two > kFaMaxSplits ? kFaMaxSplits : two) : s;
+  } else if (s == 1 && wgs <= 256 && nblk >= 32) {
+    s = 2;
+  }
+  p.splits = (int)s;
   p.part = p.splits > 1 ? wgs * p.splits * kFaWaves * (16 * D + 64) : 0;
   p.kv = (long long)B * KVH * C * D / 2;
   p.scales = ((long long)B * KVH * (2 + (C > kFaSelf ? 2 * kFaRanges : 0) + nblk) + 3) / 4 * 4;
