@@ -65,17 +65,20 @@ template <int NG, int BITS>
 Q35_DEV float fa_greatest(const uint32_t* p, int n, int C, int t, int threads) {
   constexpr float T = BITS == 4 ? 15.f : 255.f;
   float m = 0.f;
+  for (int i = 4 * t; i < n; i += 4 * threads) {
+    uint4 x[NG];  // requested together: group by group was one memory round trip each
 #pragma unroll
-  for (int g = 0; g < NG; ++g)
-    for (int i = 4 * t; i < n; i += 4 * threads) {
-      const uint4 x = *reinterpret_cast<const uint4*>(p + (size_t)g * C + i);
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    for (int g = 0; g < NG; ++g) x[g] = *reinterpret_cast<const uint4*>(p + (size_t)g * C + i);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const uint32_t w[4] = {x[g].x, x[g].y, x[g].z, x[g].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float y = fmaxf(fabsf(bf_hi(w[e])), fabsf(fmaf(T, bf_lo(w[e]), bf_hi(w[e]))));
         if (i + e < n && y < INFINITY) m = fmaxf(m, y);
       }
     }
+  }
   return m;
 }
 Q35_DEV float fa_block_max(float m, float* red) {  // of 256 threads
