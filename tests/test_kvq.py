@@ -316,6 +316,26 @@ def test_write_many_values(gpu, bits):
 
 
 @gpu_test
+@pytest.mark.parametrize("bits,dim", FORMS)
+def test_write_wide_values(gpu, bits, dim):
+    """Values of unlike exponents in a group, groups from the smallest steps to
+    the largest, few distinct values (many on the border of two codes)."""
+    g = gen(KERNEL_SEED + 936)
+    n = 96
+    x = torch.randn(3, 1, n, dim, generator=g)
+    x[0] *= torch.exp2(torch.randint(-30, 1, (1, n, dim), generator=g).float())  # unlike exponents
+    x[1] *= torch.exp2(torch.linspace(-125, 124, n))[:, None]  # every magnitude
+    x[2] = torch.randint(-40, 41, (1, n, dim), generator=g) * torch.exp2(torch.randint(-6, 7, (1, n, 1), generator=g).float())
+    k = x.to(BF)
+    v = k.flip(2).contiguous()
+    cache = to(K.quantized_kv_cache(3, 1, n, dim, bits=bits, device="cpu"), gpu)
+    K.kv_cache_quantize(k.to(gpu), v.to(gpu), cache)
+    want = cache_of(k, v, bits, n)
+    for got, w in zip(cache, want):
+        assert torch.equal(got.cpu(), w)
+
+
+@gpu_test
 @pytest.mark.parametrize("dim", [64, 256])
 def test_write_strides_and_starts(gpu, dim):
     """Token-major views, slices of a packed projection, unaligned rows, rows of
