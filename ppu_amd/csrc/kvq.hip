@@ -391,7 +391,7 @@ struct KvqShares {
   long long start;
   int s, first;
 };
-Q35_DEV KvqShares kvq_shares(const KvqArgs& a, int lane) {
+Q35_DEV KvqShares kvq_shares(const KvqShape& a, int lane) {
   KvqShares v;
   v.start = (lane < a.B ? a.len[lane] : 0) + a.offset;
   const int p = lane < a.B ? (kvq_limit(a, v.start, a.L - 1) + 127) / 128 : 0;
@@ -449,7 +449,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
     start = kvq_start(a, b);
   }
   const int bh = b * a.KVH + kvh;
-  const int G = a.G, R = a.R;
+  const int G = a.G, R = G * a.L;
 
   __shared__ alignas(1024) uint8_t lds[NW * F::RING + F::QB];
   __shared__ float ml_s[NW][HP][2];
@@ -465,7 +465,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
     if (at < F::QB) {
       const int r = min(row0 + (at + 16 * lane) / (2 * D), R - 1), i = kvq_token(a, r);
       kvq_copy(__builtin_amdgcn_readfirstlane(lds_offset(q_raw + at)),
-               (const uint8_t*)(a.q + (((size_t)b * a.QH + kvh * G + (r - i * G)) * a.L + i) * D) +
+               (const uint8_t*)(a.q + (((size_t)bh * G + (r - i * G)) * a.L + i) * D) +
                    (at + 16 * lane) % (2 * D));
     }
   }
@@ -854,7 +854,7 @@ __global__ __launch_bounds__(256, (KvqFew<D, BITS, HP>::WAVES)) void kvq_few(con
 // PER by the number of splits, after 512 tokens 7.6 us in all, with 16 always 8.0.
 constexpr int kKvqSplits = 256;
 template <int D, int HP, int PER>
-__global__ __launch_bounds__(256) void kvq_few_merge(const KvqArgs a) {
+__global__ __launch_bounds__(256) void kvq_few_merge(const KvqMergeArgs a) {
   constexpr int NW = 4, REC = HP * (D + 2);
   const int t = threadIdx.x, part = t >> 4;
   const int r = blockIdx.x / (D / 64), d = 64 * (int)(blockIdx.x % (D / 64)) + 4 * (t & 15);
@@ -878,9 +878,9 @@ __global__ __launch_bounds__(256) void kvq_few_merge(const KvqArgs a) {
   for (int j = 0; j < PER; ++j)
     x[j] = *reinterpret_cast<const float4*>(rec + (size_t)min(part + 16 * j, splits - 1) * REC + h * D + d);
   const int i = kvq_token(a, r), head = kvh * a.G + (r - i * a.G);
-  const uint2 gate = a.gate ? *reinterpret_cast<const uint2*>(a.gate + b * a.gate_stride + (2 * head + 1) * D + d)
+  const uint2 gate = a.gate ? *reinterpret_cast<const uint2*>(a.gate + (size_t)b * a.gate_stride + (2 * head + 1) * D + d)
                             : make_uint2(0, 0);
-  const int n_max = kvq_limit(a, start, kvq_token(a, min(blk * HP + HP, a.R) - 1));
+  const int n_max = kvq_limit(a, start, kvq_token(a, min(blk * HP + HP, a.G * a.L) - 1));
   const int n = min(splits, ((n_max + 31) / 32 + NW - 1) / NW);
   __shared__ float f_s[kKvqSplits], red_s[2][4];
   __shared__ float4 sum_s[16][16];
@@ -918,7 +918,7 @@ __global__ __launch_bounds__(256) void kvq_few_merge(const KvqArgs a) {
     v[0] *= sigmoid_f(bf_lo(gate.x)); v[1] *= sigmoid_f(bf_hi(gate.x));
     v[2] *= sigmoid_f(bf_lo(gate.y)); v[3] *= sigmoid_f(bf_hi(gate.y));
   }
-  *reinterpret_cast<uint2*>(a.out + (((size_t)b * a.L + i) * a.QH + head) * D + d) =
+  *reinterpret_cast<uint2*>(a.out + (((size_t)b * a.L + i) * (a.G * a.KVH) + head) * D + d) =
       make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
 }
 
@@ -1040,7 +1040,7 @@ int q35_kv_dequantize(const void* kq, const void* vq, const void* kp, const void
   const dim3 grid(((unsigned)L + 15) / 16, 2 * (unsigned)KVH, (unsigned)B);
 #define Q35_CALL(E, BITS)                                                                                          \
   kvq_read<E, BITS><<<grid, 256, 0, stream>>>((const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,          \
-                                              (const uint32_t*)vp, (uint16_t*)k, (uint16_t*)v, start, L, capacity)
+                                              (const uint32_t*)vp, (uint16_t*)k, (uint16_t*)v, start, L, KVH, capacity)
   Q35_KVQ_BY_D(Q35_CALL);
 #undef Q35_CALL
   return q35_last_error();
@@ -1061,7 +1061,7 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
   Q35_CHECK_ARG(kvq_shape_ok(B, KVH, L, D, bits, capacity) && QH > 0 && QH % KVH == 0);
   if ((long long)B * L == 0) return 0;
   Q35_CHECK_ARG(!len_dev || n_len == 1 || n_len == B);
-  Q35_CHECK_ARG(!gate || L == 1);
+  Q35_CHECK_ARG(!gate || (L == 1 && gate_stride >= 0 && gate_stride < (1ll << 31)));
   Q35_CHECK_ARG(q && kq && vq && kp && vp && out && q35_aligned16(kq) && q35_aligned16(vq) && q35_aligned16(kp) &&
                 q35_aligned16(vp) && q35_aligned16(q) && q35_aligned16(out) && q35_aligned8(gate));
   const long long rows = (long long)(QH / KVH) * L;
@@ -1069,10 +1069,11 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
   if (kvq_is_few(rows, B, KVH, L, D, capacity)) {
     const KvqFewPlan p = kvq_few_plan(B, KVH, rows, D, bits, capacity, len_dev && n_len > 1);
     Q35_CHECK_ARG(B < 65536 && KVH < 65536 && workspace && q35_aligned16(workspace) && workspace_floats >= p.floats);
-    const KvqArgs a{(const uint16_t*)q, (const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,
-                    (const uint32_t*)vp, (const long long*)len_dev, n_len, offset, (const uint16_t*)gate, gate_stride,
-                    scale, (uint16_t*)out, (float*)workspace, QH, KVH, L, capacity, p.blocks, p.splits,
-                    QH / KVH, (int)rows, B, p.share};
+    const KvqShape shape{(const long long*)len_dev, offset, n_len, KVH, L, capacity, p.blocks, p.splits, QH / KVH, B,
+                         p.share};
+    const KvqArgs a{shape, scale, (const uint16_t*)q, (const uint8_t*)kq, (const uint8_t*)vq, (const uint32_t*)kp,
+                    (const uint32_t*)vp, (float*)workspace};
+    const KvqMergeArgs m{shape, (int)gate_stride, (const float*)workspace, (const uint16_t*)gate, (uint16_t*)out};
     const long long units = (long long)B * KVH * p.splits, wgs = (units + 7) / 8 * 8 * p.blocks;
     Q35_CHECK_ARG(wgs < (1ll << 31));
     const dim3 grid = p.share ? dim3((unsigned)((p.share + B) * KVH))
@@ -1083,9 +1084,9 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
   do {                                                                             \
     if (bits == 4) kvq_few<DD, 4, HP><<<grid, 256, 0, stream>>>(a);                \
     else kvq_few<DD, 8, HP><<<grid, 256, 0, stream>>>(a);                          \
-    if (most <= 16) kvq_few_merge<DD, HP, 1><<<mgrid, 256, 0, stream>>>(a);      \
-    else if (most <= 64) kvq_few_merge<DD, HP, 4><<<mgrid, 256, 0, stream>>>(a); \
-    else kvq_few_merge<DD, HP, 16><<<mgrid, 256, 0, stream>>>(a);                  \
+    if (most <= 16) kvq_few_merge<DD, HP, 1><<<mgrid, 256, 0, stream>>>(m);      \
+    else if (most <= 64) kvq_few_merge<DD, HP, 4><<<mgrid, 256, 0, stream>>>(m); \
+    else kvq_few_merge<DD, HP, 16><<<mgrid, 256, 0, stream>>>(m);                  \
   } while (0)
     if (D == 64) Q35_FEW(64, 16);
     else if (D == 128 && hp == 8) Q35_FEW(128, 8);

@@ -18,30 +18,36 @@ Q35_DEV int kvq_shift(float x, int to) {
 
 typedef uint32_t q35_u32x2 __attribute__((ext_vector_type(2)));
 
-struct KvqArgs {
+// What the few-row kernels take, in as few bytes as it needs: a launch of 192 bytes
+// of arguments takes the host 1 us longer than one of 8.
+struct KvqShape {
+  const long long* len;
+  long long offset;
+  int n_len, KVH, L, C, blocks, splits, G, B;  // G query heads a KV head
+  int share;  // workgroups that a KV head's sequences share by their lengths; 0: `splits` for each
+};
+struct KvqArgs : KvqShape {
+  float scale;
   const uint16_t* q;
   const uint8_t *kq, *vq;
   const uint32_t *kp, *vp;
-  const long long* len;
-  int n_len;
-  long long offset;
-  const uint16_t* gate;
-  long long gate_stride;
-  float scale;
-  uint16_t* out;
   float* part;
-  int QH, KVH, L, C, blocks, splits, G, R, B;  // G = QH / KVH, R = G * L
-  int share;  // workgroups that a KV head's sequences share by their lengths; 0: `splits` for each
+};
+struct KvqMergeArgs : KvqShape {
+  int gate_stride;
+  const float* part;
+  const uint16_t* gate;
+  uint16_t* out;
 };
 
 // Row r is head r % G of token r / G; a decoded token's rows need no division.
-Q35_DEV int kvq_token(const KvqArgs& a, int r) { return a.L == 1 ? 0 : (int)((unsigned)r / (unsigned)a.G); }
+Q35_DEV int kvq_token(const KvqShape& a, int r) { return a.L == 1 ? 0 : (int)((unsigned)r / (unsigned)a.G); }
 // Keys that token i of a sequence that starts at `start` sees.
-Q35_DEV int kvq_limit(const KvqArgs& a, long long start, int i) {
+Q35_DEV int kvq_limit(const KvqShape& a, long long start, int i) {
   const long long n = start + i + 1;
   return (int)(n < 0 ? 0 : n > a.C ? a.C : n);
 }
-Q35_DEV long long kvq_start(const KvqArgs& a, int b) {
+Q35_DEV long long kvq_start(const KvqShape& a, int b) {
   return (a.len ? a.len[a.n_len > 1 ? b : 0] : 0) + a.offset;
 }
 
@@ -76,12 +82,12 @@ template <int E, int BITS>
 __global__ __launch_bounds__(256) void kvq_read(const uint8_t* __restrict__ kq, const uint8_t* __restrict__ vq,
                                                 const uint32_t* __restrict__ kp, const uint32_t* __restrict__ vp,
                                                 uint16_t* __restrict__ k, uint16_t* __restrict__ v, int start,
-                                                int L, int C) {
+                                                int L, int KVH, int C) {
   constexpr int NG = E / 4, RB = 2 * E * BITS;
   const unsigned t = blockIdx.x * 16u + (threadIdx.x >> 4);
   if (t >= (unsigned)L) return;
   const int c = threadIdx.x & 15;
-  const unsigned bh = blockIdx.z * (gridDim.y >> 1) + (blockIdx.y >> 1), pos = start + t;
+  const unsigned bh = blockIdx.z * KVH + (blockIdx.y >> 1), pos = start + t;
   const bool values = blockIdx.y & 1;
   const uint8_t* src = (values ? vq : kq) + ((size_t)bh * C + pos) * RB + c * (E * BITS / 8);
   const uint32_t* ps = (values ? vp : kp) + (size_t)bh * NG * C + pos;
