@@ -487,7 +487,7 @@ int q35_kv_dequantize(const void* kq, const void* vq, const void* kp, const void
  * sequence b sees the keys at positions 0 .. s_b + i, s_b = len_dev[b] + offset
  * (int64, n_len = B or 1 shared one; 0 + offset when len_dev is null), within
  * the capacity; a row that sees none is zero. out [B, L, QH * D] bf16. gate (L
- * == 1 only, 8-byte aligned, rows gate_stride elements apart, [q | gate] per
+ * == 1 only, 8-byte aligned, rows gate_stride (% 4 == 0) elements apart, [q | gate] per
  * query head as the packed QGKV row): out times sigmoid(gate). Workspace:
  * q35_gqa_attention_kvq_workspace floats (-1 for sizes the entry refuses), not
  * shared by launches that overlap in time. */

@@ -1061,7 +1061,7 @@ int q35_gqa_attention_kvq(const void* q, const void* kq, const void* vq, const v
   Q35_CHECK_ARG(kvq_shape_ok(B, KVH, L, D, bits, capacity) && QH > 0 && QH % KVH == 0);
   if ((long long)B * L == 0) return 0;
   Q35_CHECK_ARG(!len_dev || n_len == 1 || n_len == B);
-  Q35_CHECK_ARG(!gate || (L == 1 && gate_stride >= 0 && gate_stride < (1ll << 31)));
+  Q35_CHECK_ARG(!gate || (L == 1 && gate_stride % 4 == 0 && gate_stride >= 0 && gate_stride < (1ll << 31)));
   Q35_CHECK_ARG(q && kq && vq && kp && vp && out && q35_aligned16(kq) && q35_aligned16(vq) && q35_aligned16(kp) &&
                 q35_aligned16(vp) && q35_aligned16(q) && q35_aligned16(out) && q35_aligned8(gate));
   const long long rows = (long long)(QH / KVH) * L;

@@ -218,9 +218,9 @@ def test_refused_entries():
         a = {**ok, **kw}
         return lib.q35_kv_dequantize(*p, k, 4096, start, a["B"], a["KVH"], a["L"], a["D"], a["bits"], a["C"], None)
 
-    def attend(q=4096, QH=4, n_len=0, length=None, gate=None, ws=None, floats=0, **kw):
+    def attend(q=4096, QH=4, n_len=0, length=None, gate=None, ws=None, floats=0, gate_stride=1024, **kw):
         a = {**ok, **kw}
-        return lib.q35_gqa_attention_kvq(q, *p, length, n_len, 0, gate, 1024, 1.0, 4096, ws, floats, a["B"], QH,
+        return lib.q35_gqa_attention_kvq(q, *p, length, n_len, 0, gate, gate_stride, 1.0, 4096, ws, floats, a["B"], QH,
                                          a["KVH"], a["L"], a["D"], a["bits"], a["C"], None)
 
     for f in (write, read, attend):
@@ -233,6 +233,8 @@ def test_refused_entries():
     assert read(k=None) == 1 and read(k=4104) == 1 and read(start=62) == 1 and read(start=-1) == 1
     assert attend(q=None) == 1 and attend(q=4104) == 1 and attend(QH=3) == 1 and attend(QH=0) == 1
     assert attend(length=4096, n_len=2) == 1 and attend(gate=4096) == 1
+    assert attend(gate=4096, L=1, gate_stride=1026) == 1 and attend(gate=4096, L=1, gate_stride=-4) == 1
+    assert write(B=1 << 16) == 1 and read(B=1 << 16) == 1 and read(KVH=1 << 15) == 1
     assert lib.q35_gqa_attention_kvq_workspace(1, 3, 2, 1, 128, 4, 64) == -1
     assert lib.q35_gqa_attention_kvq_workspace(1, 4, 2, 1, 96, 4, 64) == -1
 
