@@ -659,6 +659,39 @@ def test_prefill_long(gpu, bits, dim):
 
 # ------------------------------------------------------------------ together
 @gpu_test
+@pytest.mark.parametrize("bits,dim,length,many", [(4, 256, 1, False), (8, 128, 6, False), (4, 64, 90, False),
+                                                  (4, 256, 100, True), (8, 128, 100, True), (4, 64, 200, True)])
+def test_visible_nan(gpu, bits, dim, length, many):
+    """A group of values that is NaN makes NaN of its dims, a key that is NaN of
+    every dim, for the rows that see it; the others are as without (a step of
+    bf16 apart at most: the greatest value of a head sets its power of two)."""
+    g = gen(KERNEL_SEED + 937)
+    heads, kv_heads, n = 4, 2, 230
+    capacity = roomy(heads, kv_heads, dim, length) if many else 256
+    k, v = rows(g, 1, kv_heads, n, dim), rows(g, 1, kv_heads, n, dim)
+    plain = to(cache_of(k, v, bits, capacity), gpu)
+    q = torch.randn(1, heads, length, dim, generator=g).to(BF).to(gpu)
+    want = K.gqa_prefill_attention_q(q, plain, dim**-0.5, kv_start=n - length).cpu().unflatten(-1, (heads, dim))
+    sees = torch.arange(length) + n - length
+    for at in {3, n - 1, n - length, n - length // 2 - 1}:
+        hit = sees >= at  # the rows that see position `at`
+        bad = K.QuantizedKV(*(t.clone() for t in plain))
+        bad.value_params[0, 1, 0, at] = float("nan")  # the first group of KV head 1
+        got = K.gqa_prefill_attention_q(q, bad, dim**-0.5, kv_start=n - length).cpu().unflatten(-1, (heads, dim))
+        dims = ref.groups(dim, True)[0]
+        nan = torch.zeros_like(want, dtype=torch.bool)
+        nan[:, hit, 2:] = torch.isin(torch.arange(dim), torch.as_tensor(dims))
+        assert torch.equal(torch.isnan(got), nan), f"values, position {at}"
+        torch.testing.assert_close(got[~nan].float(), want[~nan].float(), rtol=2**-7, atol=1e-6)
+        bad = K.QuantizedKV(*(t.clone() for t in plain))
+        bad.key_params[0, 0, 0, at] = float("nan")
+        got = K.gqa_prefill_attention_q(q, bad, dim**-0.5, kv_start=n - length).cpu().unflatten(-1, (heads, dim))
+        nan = torch.zeros_like(want, dtype=torch.bool)
+        nan[:, hit, :2] = True
+        assert torch.equal(torch.isnan(got), nan), f"keys, position {at}"
+
+
+@gpu_test
 def test_operators_together(gpu):
     """A prompt in two parts, then decoded tokens, as a model's attention layer
     uses them: each call's output against the oracle on the cache so far."""
