@@ -624,27 +624,38 @@ struct FaPlan {
   int tiles, splits;
   long long part, kv, scales;  // floats of the records, of K or V, of the scales, partial maxima and flags
 };
-// Ranges of a tile's keys: up to one workgroup a CU (for heads of 64, two that have
-// four blocks), as each more adds to the merge, and two for up to that many tiles
-// of a long cache, whose causal lengths would leave the early ones' CUs idle.
-// Target 256 / 512, us: 8/2 heads of 256, 1024 tokens 33.1 / 41.4, 1000 after 31768 295
-// / 306, but 3000 tokens (188 tiles) 101 / 75, 4096 (256) 132 / 109, 4096 after 28672
-// 988 / 976; 32/8 of 128, 1024 tokens (256 tiles) 32.6 / 38.9, 1000 after 3096 98.7 /
-// 99.6; 14/2 of 64, 1500 tokens 30.4 / 26.0, 1000 after 31768 235 / 190, 300 after 1748
-// (ranges of two blocks) 19.6 / 22.7.
+// Ranges of a tile's keys, at least two blocks each: the count with the least
+// estimate, in blocks of one workgroup (2.1 us in heads of 256), of
+//   the rounds of workgroups (one a CU, two in heads of 64) x the blocks of each, or
+//   the longest tile's; as the capacity is full, tiles of `avg` blocks in the mean
+//   + 3 blocks a round until the first is there (6 of the smaller heads' blocks)
+//   + the merge, by its records.
+// More tiles than a round holds are not split where most are of unequal lengths:
+// the longest start first, and splits gained nothing (6000 tokens of 8/2 heads of
+// 256, 376 tiles, one range 194 us, two 196). Fewer and more ranges, us: 1024 tokens
+// of 8/2 heads of 256 (64 tiles) two 37.0, four 33.1, eight 41.4; 3000 tokens (188)
+// one 101, two 75; 4096 (256) one 132, two 109, four 128; 748 tokens after 21874, 2
+// sequences of 12/1 heads (142) two 646, seven 464; 32/8 heads of 128, 1024 tokens (256)
+// one 32.6, two 38.9, 1200 after 15184 (304) one 566, five 425; 14/2 heads of 64, 1500
+// tokens (166) one 30.4, three 26.0.
 FaPlan fa_plan(int B, int QH, int KVH, int L, int D, int C) {
   FaPlan p;
   const long long rows = (long long)(QH / KVH) * L;
   p.tiles = (int)((rows + kFaRows - 1) / kFaRows);
   const long long wgs = (long long)p.tiles * B * KVH, nblk = (C + kFaKeys - 1) / kFaKeys;
-  long long s = 256 / wgs;
-  s = s < 1 ? 1 : s > kFaMaxSplits ? kFaMaxSplits : s;
-  s = s < (nblk + 1) / 2 ? s : (nblk + 1) / 2;
-  if (D == 64) {
-    const long long two = 512 / wgs < (nblk + 3) / 4 ? 512 / wgs : (nblk + 3) / 4;
-    s = two > s ? (two > kFaMaxSplits ? kFaMaxSplits : two) : s;
-  } else if (s == 1 && wgs <= 256 && nblk >= 32) {
-    s = 2;
+  const long long slots = D == 64 ? 512 : 256;
+  const double avg = nblk - (double)(L < C ? L : C) / (2 * kFaKeys), start = D == 256 ? 3 : 6;
+  long long s = 1;
+  if (wgs <= slots || avg >= 0.75 * nblk) {
+    double least = 0;
+    for (long long n = 1; n <= kFaMaxSplits && n <= (nblk + 1) / 2 && (n == 1 || n * wgs <= 4 * slots); ++n) {
+      const double rounds = (double)((n * wgs + slots - 1) / slots), work = rounds * avg;
+      const double t = (work > nblk ? work : (double)nblk) / n + start * rounds + (n > 1 ? start / 3 + n * wgs / 96.0 : 0);
+      if (n == 1 || t < least) {
+        least = t;
+        s = n;
+      }
+    }
   }
   p.splits = (int)s;
   p.part = p.splits > 1 ? wgs * p.splits * kFaWaves * (16 * D + 64) : 0;
