@@ -636,7 +636,7 @@ struct FaPlan {
 // of 8/2 heads of 256 (64 tiles) two 37.0, four 33.1, eight 41.4; 3000 tokens (188)
 // one 101, two 75; 4096 (256) one 132, two 109, four 128; 748 tokens after 21874, 2
 // sequences of 12/1 heads (142) two 646, seven 464; 32/8 heads of 128, 1024 tokens (256)
-// one 32.6, two 38.9, 1200 after 15184 (304) one 566, five 425; 14/2 heads of 64, 1500
+// one 32.6, two 38.9, 1200 after 15184 (304) one 566, three 425; 14/2 heads of 64, 1500
 // tokens (166) one 30.4, three 26.0.
 FaPlan fa_plan(int B, int QH, int KVH, int L, int D, int C) {
   FaPlan p;

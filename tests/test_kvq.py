@@ -692,6 +692,39 @@ def test_visible_nan(gpu, bits, dim, length, many):
 
 
 @gpu_test
+def test_far_offsets(gpu):
+    """A cache of 9.7 GB: the last of 72 sequences lies beyond 2^32 bytes of codes
+    and 2^31 values; all operators on it give what they give on that sequence
+    alone (attention: the same sums in another order, then at most one bf16 step
+    apart, 2^-7 of the value, or 1e-5, 2^-18 of the values' range)."""
+    g = gen(KERNEL_SEED + 938)
+    batch, kv_heads, dim, capacity, new = 72, 2, 256, 131072, 80
+    cache = K.quantized_kv_cache(batch, kv_heads, capacity, dim, bits=8, device=gpu)
+    for t in cache[:2]:
+        t[-1].random_(0, 256)
+    for t in cache[2:]:
+        t[-1, ..., 0], t[-1, ..., 1] = 0.01, -1.0
+    last = K.QuantizedKV(*(t[-1:].clone() for t in cache))
+    k, v = (rows(g, 1, kv_heads, new, dim).to(gpu) for _ in range(2))
+    start = torch.zeros(batch, dtype=torch.int64, device=gpu)
+    start[-1] = capacity - new
+    start[:-1] = capacity  # the others' rows are outside
+    K.kv_cache_quantize(k.expand(batch, -1, -1, -1), v.expand(batch, -1, -1, -1), cache, cache_start=start)
+    K.kv_cache_quantize(k, v, last, start=capacity - new)
+    for t, u in zip(cache, last):
+        assert torch.equal(t[-1:], u) and not t[-2].any()
+    for t, u in zip(K.kv_cache_dequantize(cache, new, start=capacity - new), K.kv_cache_dequantize(last, new, start=capacity - new)):
+        assert torch.equal(t[-1:], u) and not t[:-1].any()
+    length = torch.where(start == capacity, 0, capacity)
+    for n in (1, new):
+        q = torch.randn(1, 8, n, dim, generator=g).to(BF).to(gpu)
+        got = K.gqa_prefill_attention_q(q.expand(batch, -1, -1, -1).contiguous(), cache, dim**-0.5, valid_length=length)
+        want = K.gqa_prefill_attention_q(q, last, dim**-0.5, kv_start=capacity - n)
+        assert not got[:-1].any()
+        torch.testing.assert_close(got[-1:], want, rtol=2**-7, atol=1e-5)
+
+
+@gpu_test
 def test_operators_together(gpu):
     """A prompt in two parts, then decoded tokens, as a model's attention layer
     uses them: each call's output against the oracle on the cache so far."""
