@@ -19,6 +19,7 @@
 // Layouts: codes [B, KVH, C, D * bits / 8] bytes, dims in order, in 4 bits the
 // even dim in a byte's low half; params [B, KVH, D / 64, C] pairs of bf16
 // (step in the low half of a 32-bit word, low in the high half).
+#include <cmath>
 #include <type_traits>
 
 #include "kvq.hpp"
@@ -926,15 +927,21 @@ __global__ __launch_bounds__(256) void kvq_few_merge(const KvqMergeArgs a) {
 }
 
 // Whether the rows of a KV head go to kvq_few, which reads and unpacks the keys
-// once per block of rows, or to kvq_prompt, which unpacks them once into memory
-// and has several launches: few rows, or little work in all. Both ways, us (GPU
-// time, 4 bits): 8/2 heads of 256, 32768 tokens: 64 rows 37 / 79, 128 54 / 80,
-// 256 89 / 86, 512 159 / 90; 1024 tokens: 256 rows 15 / 25, 512 27 / 27; 32/8
-// heads of 128, 8 sequences of 32768: 64 rows 231 / 476, 128 448 / 482, 256 816
-// / 613; 14/2 heads of 64, 12 sequences of 1024: 112 rows 13 / 18, 224 20 / 20.
-// One query position is always kvq_few's, which alone applies the gate.
+// once per block of rows, or to kvq_prompt, which unpacks them once into memory and
+// has several launches: up to the rows at which unpacking a large cache pays, or
+// little work in all, where a longer cache takes kvq_prompt longer to start (both
+// borders fitted). Both ways, us (GPU time, 4 bits): 8/2 heads of 256, 512 keys: 512
+// rows 18 / 23, 1024 31 / 24; 2048 keys: 512 32 / 36, 1024 44 / 38; 8192 keys: 256 39 /
+// 55, 512 57 / 53; 32768 keys: 128 54 / 79, 512 154 / 91; 4/4 heads, 16 sequences of
+// 2048: 64 rows 61 / 72, 128 113 / 77, of 32768 64 608 / 972, 128 1103 / 973; 32/8
+// heads of 128, 8192 keys: 128 rows 25 / 38, 256 39 / 40, 8 sequences of 32768: 64 222
+// / 472, 256 764 / 608; 14/2 heads of 64, 8192 keys: 1022 rows 26 / 33, 32768 keys:
+// 511 41 / 45, 1022 70 / 50. One query position is always kvq_few's, which alone
+// applies the gate.
 bool kvq_is_few(long long rows, int B, int KVH, int L, int D, int C) {
-  return L == 1 || rows <= 128 || (double)rows * B * KVH * C * D <= (double)(1 << 28);
+  if (L == 1 || rows <= 96) return true;
+  const double work = (double)rows * B * KVH * C * D, root = std::sqrt((double)C);
+  return work <= 1.76e6 * root * std::sqrt(root) && work <= (D == 64 ? 3.0e9 : 4.29e9);  // C^(3/4)
 }
 // Rows a block of kvq_few holds: as few columns as the row count needs, as a
 // block's vector work grows with its column tiles. In heads of 256 sixteen rows

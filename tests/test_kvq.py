@@ -437,11 +437,11 @@ def test_decode_gate_many_heads(gpu):
     token is the decode kernel's at any size."""
     g = gen(KERNEL_SEED + 930)
     heads, dim, n = 144, 64, 100
-    cache = cache_of(rows(g, 1, 1, n, dim), rows(g, 1, 1, n, dim), 4, roomy(heads, 1, dim, 1), junk=float("nan"))
+    cache = cache_of(rows(g, 1, 1, n, dim), rows(g, 1, 1, n, dim), 4, 128, junk=float("nan"))
     q = torch.randn(1, heads, 1, dim, generator=g).to(BF)
     packed = (2 * torch.randn(1, 1, 2 * dim * heads, generator=g)).to(BF)
-    got = K.gqa_decode_attention_q(q.to(gpu), to(cache, gpu), torch.tensor(n, device=gpu), dim**-0.5,
-                                   packed_gate=packed.to(gpu))
+    roomier = wide(cache, roomy(heads, 1, dim, 1), gpu, float("nan"))
+    got = K.gqa_decode_attention_q(q.to(gpu), roomier, torch.tensor(n, device=gpu), dim**-0.5, packed_gate=packed.to(gpu))
     gate = packed.double().unflatten(-1, (heads, 2, dim))[..., 1, :].flatten(2)
     check_attention(got, q, cache, [n - 1], dim**-0.5, gate=torch.sigmoid(gate))
 
@@ -531,10 +531,25 @@ def test_prefill_sizes(gpu, bits, dim, heads, kv_heads, length, start):
 
 
 def roomy(heads, kv_heads, dim, length, batch=1):
-    """A capacity from which on more than 128 rows of a KV head go over the
-    unpacked cache: rows x batch x KV heads x capacity x dim above 2^28."""
-    capacity = (1 << 28) // (heads // kv_heads * length * batch * kv_heads * dim) + 1
+    """A capacity at which more than 96 rows of a KV head go over the unpacked
+    cache whatever it is: rows x batch x KV heads x capacity x dim above 2^32
+    (heads of 64: 2^31.5)."""
+    capacity = int(2 ** (31.5 if dim == 64 else 32)) // (heads // kv_heads * length * batch * kv_heads * dim) + 1
     return (capacity + 31) // 32 * 32
+
+
+def wide(cache, capacity, device, junk=0.0):
+    """``cache`` on the GPU with ``capacity`` positions, the codes of the others
+    all ones and their params ``junk``."""
+    out = []
+    for t in cache:
+        dim, fill = (2, 255) if t.ndim == 4 else (3, junk)
+        shape = list(t.shape)
+        shape[dim] = capacity
+        w = torch.full(shape, fill, dtype=t.dtype, device=device)
+        w.narrow(dim, 0, t.shape[dim]).copy_(t)
+        out.append(w)
+    return K.QuantizedKV(*out)
 
 
 @gpu_test
@@ -545,14 +560,15 @@ def test_prefill_many_rows(gpu, bits, dim, heads, kv_heads, length, start):
     """Row tiles that end inside a token, in the middle of a wave, in several
     tiles; key ranges of one and several blocks; the rest of the cache NaN."""
     g = gen(KERNEL_SEED + 916)
-    n, capacity = start + length, roomy(heads, kv_heads, dim, length)
+    n = start + length
     k, v = rows(g, 1, kv_heads, n, dim), rows(g, 1, kv_heads, n, dim)
-    cache = cache_of(k, v, bits, capacity, junk=float("nan"))
+    cache = cache_of(k, v, bits, (n + 31) // 32 * 32, junk=float("nan"))
     q = torch.randn(1, heads, length, dim, generator=g).to(BF)
-    got = K.gqa_prefill_attention_q(q.to(gpu), to(cache, gpu), dim**-0.5, kv_start=start)
+    roomier = wide(cache, roomy(heads, kv_heads, dim, length), gpu, float("nan"))
+    got = K.gqa_prefill_attention_q(q.to(gpu), roomier, dim**-0.5, kv_start=start)
     check_attention(got, q, cache, [start], dim**-0.5, prompt=True)
     valid = torch.tensor([start], device=gpu)
-    again = K.gqa_prefill_attention_q(q.to(gpu), to(cache, gpu), dim**-0.5, valid_length=valid, length_is_start=True)
+    again = K.gqa_prefill_attention_q(q.to(gpu), roomier, dim**-0.5, valid_length=valid, length_is_start=True)
     assert torch.equal(got, again)
 
 
@@ -564,14 +580,14 @@ def test_prefill_many_rows_magnitudes(gpu, bits, dim, scale_k, scale_v):
     one row of queries is zero and one has a value 2^20 above the others."""
     g = gen(KERNEL_SEED + 917)
     heads, length = 4, 64
-    capacity = roomy(heads, 1, dim, length)
     k, v = rows(g, 1, 1, length, dim), rows(g, 1, 1, length, dim)
-    cache = cache_of((k.float() * scale_k).to(BF), (v.float() * scale_v).to(BF), bits, capacity)
+    cache = cache_of((k.float() * scale_k).to(BF), (v.float() * scale_v).to(BF), bits, length)
     q = (torch.randn(1, heads, length, dim, generator=g) / scale_k).to(BF)
     q[0, 1, 5] = 0
     q[0, 2, 9] *= 2.0**-20
     q[0, 2, 9, 3] = 1 / scale_k
-    got = K.gqa_prefill_attention_q(q.to(gpu), to(cache, gpu), dim**-0.5).double().cpu() / scale_v
+    roomier = wide(cache, roomy(heads, 1, dim, length), gpu)
+    got = K.gqa_prefill_attention_q(q.to(gpu), roomier, dim**-0.5).double().cpu() / scale_v
     # the oracle on the same numbers, brought back in 64 bits
     kd, vd = values_of(cache)
     want = ref.attend(q.double() * scale_k, kd / scale_k, vd / scale_v, [0], dim**-0.5)
@@ -582,25 +598,27 @@ def test_prefill_many_rows_magnitudes(gpu, bits, dim, scale_k, scale_v):
 
 
 @gpu_test
-@pytest.mark.parametrize("bits,dim,length", [(4, 256, 100), (8, 128, 100), (4, 64, 150)])
-@pytest.mark.parametrize("roomier", [1, 4])
-def test_prefill_batch_many_rows(gpu, bits, dim, length, roomier):
-    """As test_prefill_batch, over the unpacked cache, in short caches and in
-    ones whose greatest values are found by a launch of its own."""
+@pytest.mark.parametrize("bits,dim,length,heads,capacity", [
+    (4, 256, 100, 4, None), (8, 128, 100, 4, None), (4, 64, 150, 4, None),
+    (4, 256, 100, 16, 768), (8, 128, 150, 16, 768), (4, 64, 150, 32, 768), (8, 256, 130, 24, 2048)])
+def test_prefill_batch_many_rows(gpu, bits, dim, length, heads, capacity):
+    """As test_prefill_batch, over the unpacked cache: in roomy caches, whose
+    greatest values are found by a launch of its own, and in short ones."""
     g = gen(KERNEL_SEED + 918)
-    capacity = roomier * roomy(4, 2, dim, length, 4)
+    capacity = capacity or roomy(heads, 2, dim, length, 4)
     n = 256
     starts = [0, 77, -length // 2, n - length]
-    cache = cache_of(rows(g, 4, 2, n, dim), rows(g, 4, 2, n, dim), bits, capacity, junk=float("inf"))
+    cache = cache_of(rows(g, 4, 2, n, dim), rows(g, 4, 2, n, dim), bits, n)
     for b, s in enumerate(starts):
         cache.key_params[b, :, :, max(s + length, 0) :] = float("nan")
         cache.value_params[b, :, :, max(s + length, 0) :] = float("nan")
     # the keys of the last token NaN in one sequence, a group of its values in another
     cache.key_params[0, :, :, length - 1] = float("nan")
     cache.value_params[1, :, 0, 77 + length - 1] = float("nan")
-    q = torch.randn(4, 4, length, dim, generator=g).to(BF)
+    q = torch.randn(4, heads, length, dim, generator=g).to(BF)
     valid = torch.tensor([s + length for s in starts], device=gpu)
-    got = K.gqa_prefill_attention_q(q.to(gpu), to(cache, gpu), dim**-0.5, valid_length=valid).cpu()
+    roomier = wide(cache, capacity, gpu, float("inf"))
+    got = K.gqa_prefill_attention_q(q.to(gpu), roomier, dim**-0.5, valid_length=valid).cpu()
     kd, vd = values_of(cache)
     assert torch.isnan(got[0, -1]).all()
     want = ref.attend(q[1:2], kd[1:2], vd[1:2], [77], dim**-0.5)[0, -1]
@@ -650,10 +668,10 @@ def test_prefill_long(gpu, bits, dim):
     g = gen(KERNEL_SEED + 912)
     length, start = 67, 5000
     n = start + length
-    capacity = max(5088, roomy(4, 1, dim, length))
-    cache = cache_of(rows(g, 1, 1, n, dim), rows(g, 1, 1, n, dim), bits, capacity, junk=float("nan"))
+    cache = cache_of(rows(g, 1, 1, n, dim), rows(g, 1, 1, n, dim), bits, 5088, junk=float("nan"))
     q = torch.randn(1, 4, length, dim, generator=g).to(BF)
-    got = K.gqa_prefill_attention_q(q.to(gpu), to(cache, gpu), dim**-0.5, kv_start=start)
+    roomier = wide(cache, roomy(4, 1, dim, length), gpu, float("nan"))
+    got = K.gqa_prefill_attention_q(q.to(gpu), roomier, dim**-0.5, kv_start=start)
     check_attention(got, q, cache, [start], dim**-0.5, prompt=True)
 
 
@@ -667,9 +685,8 @@ def test_visible_nan(gpu, bits, dim, length, many):
     bf16 apart at most: the greatest value of a head sets its power of two)."""
     g = gen(KERNEL_SEED + 937)
     heads, kv_heads, n = 4, 2, 230
-    capacity = roomy(heads, kv_heads, dim, length) if many else 256
     k, v = rows(g, 1, kv_heads, n, dim), rows(g, 1, kv_heads, n, dim)
-    plain = to(cache_of(k, v, bits, capacity), gpu)
+    plain = wide(cache_of(k, v, bits, 256), roomy(heads, kv_heads, dim, length) if many else 256, gpu)
     q = torch.randn(1, heads, length, dim, generator=g).to(BF).to(gpu)
     want = K.gqa_prefill_attention_q(q, plain, dim**-0.5, kv_start=n - length).cpu().unflatten(-1, (heads, dim))
     sees = torch.arange(length) + n - length
@@ -851,8 +868,8 @@ def test_two_streams(gpu):
     g = gen(KERNEL_SEED + 915)
     jobs = []
     for heads, kv_heads, dim, length in ((8, 2, 256, 1), (4, 1, 128, 65)):
-        cache = to(cache_of(rows(g, 2, kv_heads, 900, dim), rows(g, 2, kv_heads, 900, dim), 4,
-                            roomy(heads, kv_heads, dim, length, 2) if length > 1 else 928), gpu)
+        cache = wide(cache_of(rows(g, 2, kv_heads, 900, dim), rows(g, 2, kv_heads, 900, dim), 4, 928),
+                     roomy(heads, kv_heads, dim, length, 2) if length > 1 else 928, gpu)
         q = torch.randn(2, heads, length, dim, generator=g).to(BF).to(gpu)
         valid = torch.tensor([900, 411], device=gpu)
         jobs.append((q, cache, valid, dim**-0.5))
