@@ -5,13 +5,14 @@
 // A row tile of 128 rows reads every key once, so a prompt of n rows would
 // unpack a cache n / 128 times inside the attention; unpacked once, its blocks
 // go from memory straight into LDS. 4096 tokens after 28000 (8/2 heads of 256, 8
-// bits) take 970 us, 27 of them unpacking and 13 the merge of two ranges: 1040
-// TFLOP/s in all, where a large library product reaches 1384. The values are held in 16 bits as fp16 times
-// one power of two per head that brings the greatest of them (by the params,
-// over the keys that are seen) to 2^14: 11 significant bits down to 2^-28 of it,
-// 2^-12 off at most (bf16 would be 2^-8, more than an 8-bit cache's own step).
-// Queries are exact in fp16 times a power of two of their row, but for values
-// below 2^-21 of its greatest.
+// bits) take 947 to 970 us, 27 of them unpacking and 13 the merge of two ranges:
+// 1040 TFLOP/s and more in all, where a large library product reaches 1384.
+//
+// The values are held in 16 bits as fp16 times one power of two per head that
+// brings the greatest of them (by the params, over the keys that are seen) to
+// 2^14: 11 significant bits down to 2^-28 of it, 2^-12 off at most (bf16 would be
+// 2^-8, more than an 8-bit cache's own step). Queries are exact in fp16 times a
+// power of two of their row, but for values below 2^-21 of its greatest.
 #include "kvq.hpp"
 
 namespace {
